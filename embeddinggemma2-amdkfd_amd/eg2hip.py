@@ -102,6 +102,45 @@ class EgSaxpy(C.Structure):
     _fields_ = [("y", _vp), ("x", _vp), ("a", C.c_float), ("n", _u)]
 
 
+# The records of the block operators (include/eg2_hip.h) and the ids of their types and activations.
+_u64 = C.c_uint64
+TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
+ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3}
+
+
+class LinearArgs(C.Structure):
+    """eg2_linear_args."""
+    _fields_ = [("y", _vp), ("x", _vp), ("weight", _vp), ("bias", _vp), ("residual", _vp), ("ldx", _u64),
+                ("ldw", _u64), ("ldy", _u64), ("ldr", _u64), ("n", _u), ("k", _u), ("m", _u), ("type", _u),
+                ("weight_type", _u), ("act", _u)]
+
+
+class LinearGatedArgs(C.Structure):
+    """eg2_linear_gated_args."""
+    _fields_ = [("y", _vp), ("x", _vp), ("gate", _vp), ("up", _vp), ("gate_bias", _vp), ("up_bias", _vp),
+                ("ldx", _u64), ("ldw", _u64), ("ldy", _u64), ("n", _u), ("k", _u), ("m", _u), ("type", _u),
+                ("weight_type", _u), ("act", _u)]
+
+
+class HeadsNormRopeArgs(C.Structure):
+    """eg2_heads_norm_rope_args."""
+    _fields_ = [("q_out", _vp), ("k_out", _vp), ("q", _vp), ("k", _vp), ("q_weight", _vp), ("k_weight", _vp),
+                ("table", _vp), ("pos", _vp), ("q_row", _u64), ("q_head", _u64), ("k_row", _u64), ("k_head", _u64),
+                ("q_out_row", _u64), ("q_out_head", _u64), ("k_out_row", _u64), ("k_out_head", _u64), ("rows", _u),
+                ("q_heads", _u), ("k_heads", _u), ("d", _u), ("rotary", _u), ("table_rows", _u), ("type", _u),
+                ("eps", C.c_float), ("q_scale", C.c_float)]
+
+
+class WindowAttentionArgs(C.Structure):
+    """eg2_window_attention_args."""
+    _fields_ = [("out", _vp), ("q", _vp), ("k", _vp), ("v", _vp), ("q_offsets", _vp), ("k_offsets", _vp),
+                ("k_lengths", _vp), ("workspace", _vp), ("workspace_bytes", _u64), ("q_row", _u64), ("q_head", _u64),
+                ("k_row", _u64), ("k_head", _u64), ("v_row", _u64), ("v_head", _u64), ("out_row", _u64),
+                ("out_head", _u64), ("batch", _u), ("rows", _u), ("key_rows", _u), ("heads", _u), ("kv_heads", _u),
+                ("d", _u), ("type", _u), ("left", C.c_int), ("right", C.c_int), ("sinks", _u), ("longest", _u),
+                ("scale", C.c_float)]
+
+
 # Every symbol declared in include/eg2_hip.h, eg2_ops.h, eg2_stream.h and gemma2_kfd.h.
 SIGNATURES = {
     "eg2_op_launch": (C.c_int, [C.c_char_p, _vp, C.c_size_t, _u, _u, _u, _vp]),
@@ -130,6 +169,11 @@ SIGNATURES = {
     "eg2_hip_gemm_q8_geglu": (C.c_int, [_vp, _vp, _u, _vp, _vp, _u, _vp, _vp, _u, _u, _u, _u, _vp]),
     "eg2_hip_gemm_q8_qkv_rope": (C.c_int, [_vp, _vp, _u, _vp, _vp, _u, _u, _u, _vp, _vp, _vp, _vp, C.c_float, _vp,
                                            _vp]),
+    "eg2_hip_linear": (C.c_int, [C.POINTER(LinearArgs), _vp]),
+    "eg2_hip_linear_gated": (C.c_int, [C.POINTER(LinearGatedArgs), _vp]),
+    "eg2_hip_heads_norm_rope": (C.c_int, [C.POINTER(HeadsNormRopeArgs), _vp]),
+    "eg2_hip_window_attention": (C.c_int, [C.POINTER(WindowAttentionArgs), _vp]),
+    "eg2_hip_window_attention_workspace": (C.c_uint64, [C.POINTER(WindowAttentionArgs)]),
     "eg2_hip_error_string": (C.c_char_p, [C.c_int]),
     "eg2_hip_device_check": (C.c_int, [C.c_char_p, C.c_size_t]),
     "eg2_q8_tile_bytes": (C.c_size_t, [C.c_size_t, _u]),
@@ -738,3 +782,210 @@ class ops:
         check(lib().eg2_hip_gemm_q8_geglu(cls._p(xq), cls._p(xd), xd.shape[1], cls._p(wq), cls._p(wd), wd.shape[1],
                                           cls._p(gq), cls._p(gd), gd.shape[1], n, ff, k, cls._stream()),
               "gemm_q8_geglu")
+
+    # ---- block operators: any geometry, fp32 / fp16 / bf16 (include/eg2_hip.h). They run on the current
+    # stream of their tensors' device.
+
+    @staticmethod
+    def _type(t, what):
+        """The id of an activation tensor's type."""
+        import torch
+
+        types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        if t.dtype not in types:
+            raise ValueError(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
+        return types[t.dtype]
+
+    @staticmethod
+    def _on(what, device, **tensors):
+        """Every tensor that is given lies on the GPU `device`."""
+        if device.type != "cuda":
+            raise ValueError(f"{what}: tensors on {device}, not on a GPU")
+        for name, t in tensors.items():
+            if t is not None and t.device != device:
+                raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+
+    @staticmethod
+    def _row_stride(t, what, name):
+        """Elements between the rows of a matrix whose rows are dense."""
+        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+            raise ValueError(f"{what}: {name} is no matrix of dense rows")
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+    @staticmethod
+    def _head_strides(t, what, name):
+        """Elements between the rows and the heads of [rows, heads, d] with dense heads."""
+        if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+            raise ValueError(f"{what}: {name} is not [rows, heads, d] with dense heads")
+        head = t.stride(1) if t.shape[1] > 1 else t.shape[2]
+        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * head, head
+
+    @staticmethod
+    def _vector(t, what, name, n, dtype):
+        """A dense vector of n values of a type, if given."""
+        if t is not None and (t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or not t.is_contiguous()):
+            raise ValueError(f"{what}: {name} is not {n} dense values of {dtype}")
+
+    @classmethod
+    def _launch(cls, what, entry, args, device):
+        import torch
+
+        if torch.cuda.current_device() == device.index:
+            check(entry(C.byref(args), cls._stream()), what)
+        else:
+            with torch.cuda.device(device):
+                check(entry(C.byref(args), cls._stream()), what)
+
+    @classmethod
+    def _weights(cls, what, w, name, m, k, x):
+        """(type id, row stride in values) of [m, k] weights: uint8 tensors hold rows of Q8_0 blocks."""
+        import torch
+
+        ld = cls._row_stride(w, what, name)
+        if w.dtype == torch.uint8:
+            if k % 32 or tuple(w.shape) != (m, k // 32 * 34) or ld % 34:
+                raise ValueError(f"{what}: {name} is not {m} rows of {k} Q8_0 values (whole blocks of 34 bytes)")
+            return TYPE_Q8_0, ld // 34 * 32
+        if tuple(w.shape) != (m, k):
+            raise ValueError(f"{what}: {name} is {tuple(w.shape)}, not {(m, k)}")
+        if x.dtype != torch.float32 and w.dtype != x.dtype:
+            raise ValueError(f"{what}: {name} of {w.dtype} with activations of {x.dtype}")
+        return cls._type(w, what), ld
+
+    @classmethod
+    def linear(cls, x, weight, y, bias=None, act="none", residual=None):
+        """y = act(x . weight^T + bias) + residual (eg2_hip_linear): x [n, k],
+        weight [m, k] or uint8 [m, 34 k / 32] of Q8_0 blocks, y [n, m], bias
+        float32 [m], residual [n, m] (may be y); act "none", "gelu", "silu" or "relu"."""
+        import torch
+
+        what = "linear"
+        kind, ldx, ldy = cls._type(x, what), cls._row_stride(x, what, "x"), cls._row_stride(y, what, "y")
+        (n, k), m = x.shape, y.shape[1]
+        if y.shape[0] != n or y.dtype != x.dtype:
+            raise ValueError(f"{what}: y is {tuple(y.shape)} of {y.dtype}, not {n} rows of {x.dtype}")
+        wtype, ldw = cls._weights(what, weight, "weight", m, k, x)
+        cls._vector(bias, what, "bias", m, torch.float32)
+        ldr = 0
+        if residual is not None:
+            ldr = cls._row_stride(residual, what, "residual")
+            if residual.shape != y.shape or residual.dtype != y.dtype:
+                raise ValueError(f"{what}: residual is not of y's shape and type")
+        if act not in ACTIVATIONS:
+            raise ValueError(f"{what}: no activation {act!r}")
+        cls._on(what, x.device, weight=weight, y=y, bias=bias, residual=residual)
+        args = LinearArgs(cls._p(y), cls._p(x), cls._p(weight), cls._p(bias), cls._p(residual), ldx, ldw, ldy, ldr, n,
+                          k, m, kind, wtype, ACTIVATIONS[act])
+        cls._launch(what, lib().eg2_hip_linear, args, x.device)
+
+    @classmethod
+    def linear_gated(cls, x, gate, up, y, gate_bias=None, up_bias=None, act="gelu"):
+        """y = act(x . gate^T + gate_bias) * (x . up^T + up_bias)
+        (eg2_hip_linear_gated): the arguments of linear, gate and up alike."""
+        import torch
+
+        what = "linear_gated"
+        kind, ldx, ldy = cls._type(x, what), cls._row_stride(x, what, "x"), cls._row_stride(y, what, "y")
+        (n, k), m = x.shape, y.shape[1]
+        if y.shape[0] != n or y.dtype != x.dtype:
+            raise ValueError(f"{what}: y is {tuple(y.shape)} of {y.dtype}, not {n} rows of {x.dtype}")
+        wtype, ldw = cls._weights(what, gate, "gate", m, k, x)
+        if cls._weights(what, up, "up", m, k, x) != (wtype, ldw):
+            raise ValueError(f"{what}: gate and up differ in type or stride")
+        cls._vector(gate_bias, what, "gate_bias", m, torch.float32)
+        cls._vector(up_bias, what, "up_bias", m, torch.float32)
+        if act not in ACTIVATIONS:
+            raise ValueError(f"{what}: no activation {act!r}")
+        cls._on(what, x.device, gate=gate, up=up, y=y, gate_bias=gate_bias, up_bias=up_bias)
+        args = LinearGatedArgs(cls._p(y), cls._p(x), cls._p(gate), cls._p(up), cls._p(gate_bias), cls._p(up_bias), ldx,
+                               ldw, ldy, n, k, m, kind, wtype, ACTIVATIONS[act])
+        cls._launch(what, lib().eg2_hip_linear_gated, args, x.device)
+
+    @classmethod
+    def heads_norm_rope(cls, q, k, q_w, k_w, table, pos, eps, q_out, k_out, q_scale=1.0):
+        """Every head of q [rows, heads, d] and k [rows, kv_heads, d] (k and
+        k_out may be None) RMS-normalised, times q_w / k_w (float32 [d] or None),
+        rotated by table[pos] (float32 [positions, rotary] as rope_table, int32
+        [rows]; both None: not rotated) and, of q, scaled, into q_out and k_out,
+        which may be q and k (eg2_hip_heads_norm_rope)."""
+        import torch
+
+        what = "heads_norm_rope"
+        rows, heads, d = q.shape if q.dim() == 3 else (0, 0, 0)
+        args = HeadsNormRopeArgs(type=cls._type(q, what), rows=rows, q_heads=heads, d=d, eps=eps, q_scale=q_scale,
+                                 q=cls._p(q), q_out=cls._p(q_out), q_weight=cls._p(q_w))
+        args.q_row, args.q_head = cls._head_strides(q, what, "q")
+        args.q_out_row, args.q_out_head = cls._head_strides(q_out, what, "q_out")
+        if q_out.shape != q.shape or q_out.dtype != q.dtype:
+            raise ValueError(f"{what}: q_out is not of q's shape and type")
+        cls._vector(q_w, what, "q_w", d, torch.float32)
+        if (k is None) != (k_out is None):
+            raise ValueError(f"{what}: k and k_out go together")
+        if k is not None:
+            args.k_row, args.k_head = cls._head_strides(k, what, "k")
+            args.k_out_row, args.k_out_head = cls._head_strides(k_out, what, "k_out")
+            if k.shape[0] != rows or k.shape[2] != d or k.dtype != q.dtype:
+                raise ValueError(f"{what}: k is {tuple(k.shape)} of {k.dtype}, not {rows} rows of heads of {d}, {q.dtype}")
+            if k_out.shape != k.shape or k_out.dtype != k.dtype:
+                raise ValueError(f"{what}: k_out is not of k's shape and type")
+            cls._vector(k_w, what, "k_w", d, torch.float32)
+            args.k_heads, args.k, args.k_out, args.k_weight = k.shape[1], cls._p(k), cls._p(k_out), cls._p(k_w)
+        if (table is None) != (pos is None):
+            raise ValueError(f"{what}: table and pos go together")
+        if table is not None:
+            if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+                raise ValueError(f"{what}: table is not a dense float32 matrix")
+            cls._vector(pos, what, "pos", rows, torch.int32)
+            args.table, args.pos, args.table_rows, args.rotary = cls._p(table), cls._p(pos), *table.shape
+        cls._on(what, q.device, k=k, q_w=q_w, k_w=k_w, table=table, pos=pos, q_out=q_out, k_out=k_out)
+        cls._launch(what, lib().eg2_hip_heads_norm_rope, args, q.device)
+
+    @classmethod
+    def window_attention(cls, q, k, v, q_offsets, k_offsets, out, scale, left=-1, right=-1, sinks=0, k_lengths=None,
+                         longest=0, workspace=None):
+        """out = attention of q [rows, heads, d] over k and v [key rows,
+        kv_heads, d] of the sequences that the int32 offsets (and lengths of keys) give,
+        each query seeing `left` keys before its own, `right` after it (-1: all)
+        and the first `sinks` (eg2_hip_window_attention). longest: the longest
+        sequence of keys, a hint. workspace: a uint8 tensor of
+        window_attention_workspace's bytes; by default one is taken from torch."""
+        import torch
+
+        what = "window_attention"
+        if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or out.shape != q.shape or k.shape[2] != q.shape[2]:
+            raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and out "
+                             f"{tuple(out.shape)} do not fit")
+        if not q.dtype == k.dtype == v.dtype == out.dtype:
+            raise ValueError(f"{what}: q, k, v and out differ in type")
+        batch = q_offsets.numel() - 1
+        for name, t, n in (("q_offsets", q_offsets, batch + 1), ("k_offsets", k_offsets, batch + 1),
+                           ("k_lengths", k_lengths, batch)):
+            cls._vector(t, what, name, n, torch.int32)
+        cls._on(what, q.device, k=k, v=v, out=out, q_offsets=q_offsets, k_offsets=k_offsets, k_lengths=k_lengths,
+                workspace=workspace)
+        args = WindowAttentionArgs(cls._p(out), cls._p(q), cls._p(k), cls._p(v), cls._p(q_offsets), cls._p(k_offsets),
+                                   cls._p(k_lengths), None, 0, *cls._head_strides(q, what, "q"),
+                                   *cls._head_strides(k, what, "k"), *cls._head_strides(v, what, "v"),
+                                   *cls._head_strides(out, what, "out"), max(batch, 0), q.shape[0], k.shape[0],
+                                   q.shape[1], k.shape[1], q.shape[2], cls._type(q, what), left, right, sinks, longest,
+                                   scale)
+        need = lib().eg2_hip_window_attention_workspace(C.byref(args))
+        if workspace is None and need:  # torch keeps it for this stream until the kernels are done
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        if workspace is not None:
+            if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
+                raise ValueError(f"{what}: workspace is not a dense uint8 tensor")
+            args.workspace, args.workspace_bytes = cls._p(workspace), workspace.numel()
+        cls._launch(what, lib().eg2_hip_window_attention, args, q.device)
+
+    @classmethod
+    def window_attention_workspace(cls, batch, rows, key_rows, heads, kv_heads, d, dtype, left=-1, right=-1, sinks=0,
+                                   longest=0):
+        """Bytes of workspace of a window_attention call of these sizes."""
+        import torch
+
+        types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
+        args = WindowAttentionArgs(batch=batch, rows=rows, key_rows=key_rows, heads=heads, kv_heads=kv_heads, d=d,
+                                   type=types.get(dtype, 0xffffffff), left=left, right=right, sinks=sinks,
+                                   longest=longest)
+        return lib().eg2_hip_window_attention_workspace(C.byref(args))

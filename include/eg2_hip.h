@@ -218,6 +218,125 @@ int eg2_hip_gemm_q8_geglu(const int8_t *xq, const float *xd, unsigned ldx, const
                           unsigned ldw, int8_t *gq, float *gd, unsigned ldg, unsigned n, unsigned ff, unsigned k,
                           void *stream);
 
+/* ------------------------------------------------------------ block operators
+ * Floating-point operators of a transformer block, in any geometry, for
+ * activations of fp32, fp16 or bf16. They have no counterpart in the
+ * reference, whose operators take fp32 activations in fixed head geometries;
+ * they stand beside eg2_op_launch's projections, norms and attention. Each
+ * takes its arguments by a record (copied before the call returns) and a
+ * stream of the current device, enqueues its kernels and returns 0 or a
+ * hipError_t code; hipErrorInvalidValue for a record that breaks a rule below,
+ * with nothing launched. They allocate nothing, keep nothing from one call to
+ * the next and can be captured into a HIP graph. Sums, softmax statistics and
+ * norms are held in 32 bits; every result is rounded once to its type (the
+ * softmax weights of 16-bit attention also, before they multiply the values).
+ * Strides count elements and are free for inputs (0 repeats a row); pointers lie on their
+ * type's own alignment (Q8_0 blocks on 2 bytes). An output overlaps no input unless its
+ * rule says so. */
+
+/* Element types, by their GGML ids as in EgMM. */
+#define EG2_TYPE_F32 0u
+#define EG2_TYPE_F16 1u
+#define EG2_TYPE_Q8_0 8u
+#define EG2_TYPE_BF16 30u
+
+#define EG2_ACT_NONE 0u
+#define EG2_ACT_GELU 1u /* tanh form: z / (1 + exp(-2 s z (1 + a z^2))), s = sqrt(2 / pi), a = 0.044715 */
+#define EG2_ACT_SILU 2u /* z / (1 + exp(-z)) */
+#define EG2_ACT_RELU 3u /* max(z, 0), NaN stays */
+
+/* y[n][m] = act(x[n][k] . weight[m][k]^T + bias[m]) + residual[n][m].
+ * x, y and residual are of `type` (F32, F16 or BF16); weight of weight_type: Q8_0,
+ * the same type, or with F32 activations any of the four. Q8_0 rows are k / 32
+ * blocks of 34 bytes, ldw / 32 blocks apart (k and ldw multiples of 32). bias
+ * (fp32) and residual may be NULL; residual may be y itself with the same
+ * stride. n, k, m: 1 to 2^24, n m at most 2^32; ldy >= m. An output's bits follow from its own row and
+ * column and from n, k, m, the types and the operands' alignment. */
+typedef struct {
+    void *y;
+    const void *x, *weight;
+    const float *bias;
+    const void *residual;
+    uint64_t ldx, ldw, ldy, ldr;
+    unsigned n, k, m, type, weight_type, act;
+} eg2_linear_args;
+int eg2_hip_linear(const eg2_linear_args *args, void *stream);
+
+/* The gated half of a feed-forward block, both projections in one kernel:
+ * y[n][m] = act(x . gate^T + gate_bias) * (x . up^T + up_bias), the rules of
+ * eg2_hip_linear; gate and up are of one type and stride. */
+typedef struct {
+    void *y;
+    const void *x, *gate, *up;
+    const float *gate_bias, *up_bias;
+    uint64_t ldx, ldw, ldy;
+    unsigned n, k, m, type, weight_type, act;
+} eg2_linear_gated_args;
+int eg2_hip_linear_gated(const eg2_linear_gated_args *args, void *stream);
+
+/* The norms of queries and keys for each head, with the position rotation, in
+ * one pass: for every row r and head, u = x / sqrt(mean(x^2) + eps) * weight,
+ * then the pairs (i, i + rotary/2), i < rotary/2, are rotated by the angle whose
+ * cosine and sine are table[pos[r]][i] and table[pos[r]][rotary/2 + i] (fp32,
+ * eg2_rope_table's layout, table_rows rows of `rotary` floats); the other values of
+ * the head pass, and q is multiplied by q_scale. q has q_heads heads, k k_heads
+ * (0: k is absent); element e of head h of row r lies at r * row stride + h *
+ * head stride + e. q_out and k_out may be q and k themselves with the same
+ * strides. The weights ([d], fp32) may be NULL (1). A row whose position is not
+ * in [0, table_rows) comes out as NaN. d: even, 2 to 512; rotary: even, at most d (0: no
+ * rotation, table and pos may be NULL); rows: 1 to 2^24; at most 4096 heads in all. */
+typedef struct {
+    void *q_out, *k_out;
+    const void *q, *k;
+    const float *q_weight, *k_weight, *table;
+    const int32_t *pos;
+    uint64_t q_row, q_head, k_row, k_head, q_out_row, q_out_head, k_out_row, k_out_head;
+    unsigned rows, q_heads, k_heads, d, rotary, table_rows, type;
+    float eps, q_scale;
+} eg2_heads_norm_rope_args;
+int eg2_hip_heads_norm_rope(const eg2_heads_norm_rope_args *args, void *stream);
+
+/* Attention over a sliding window and a few first keys that stay visible, for
+ * packed sequences, prompts over a cache and single tokens:
+ * out[r][h] = sum_s softmax_s(scale q[r][h] . k[s][g]) v[s][g], g = h /
+ * (heads / kv_heads), over the keys s that r sees. Sequence b has the query rows
+ * [q_offsets[b], q_offsets[b+1]) and the key rows k_offsets[b] + s, 0 <= s < L,
+ * L = k_offsets[b+1] - k_offsets[b], or k_lengths[b] where k_lengths is not NULL (at
+ * most that difference). The last query stands at the last key: query i of n has
+ * position p = L - n + i, and sees key s iff
+ *   (right < 0 or s <= p + right) and (left < 0 or s >= p - left or s < sinks).
+ * (right = 0: causal; left = right = w / 2: the executor's window w.) A row
+ * that sees no key is 0; a key that a row does not see does not touch it,
+ * whatever it holds. Rows of q that are in no sequence are left as they are in out,
+ * and so is every row of a sequence without queries. Offsets (device, batch + 1,
+ * not descending) are clipped to `rows` and `key_rows`, the rows of q and of k
+ * and v that may be touched. q, k, v and out are of `type`, F32, F16 or BF16;
+ * d: a multiple of 8, 8 to 256; their pointers lie on 16 bytes and their strides are
+ * multiples of 16 bytes. heads is a multiple of kv_heads, at most 4096. batch: 1 to 65535;
+ * rows and key_rows: 1 to 2^31 - 1. longest: the longest
+ * sequence of keys (0: unknown), a hint: it chooses how the keys of few queries are
+ * split over the GPU, which costs time or the order of sums, never a key. workspace: device memory of
+ * at least eg2_hip_window_attention_workspace(args) bytes (which may be 0), 16-byte
+ * aligned, used by this call until its kernels are done: two calls that may
+ * run at the same time, and two captured graphs that may, have one each.
+ * scale: finite. */
+typedef struct {
+    void *out;
+    const void *q, *k, *v;
+    const int32_t *q_offsets, *k_offsets, *k_lengths;
+    void *workspace;
+    uint64_t workspace_bytes;
+    uint64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+    unsigned batch, rows, key_rows, heads, kv_heads, d, type;
+    int left, right;
+    unsigned sinks, longest;
+    float scale;
+} eg2_window_attention_args;
+int eg2_hip_window_attention(const eg2_window_attention_args *args, void *stream);
+/* Bytes of workspace the call needs (0 for a record it rejects); from the sizes, `type` and
+ * `longest` alone: no pointer is looked at. */
+uint64_t eg2_hip_window_attention_workspace(const eg2_window_attention_args *args);
+
 /* ------------------------------------------------------------ executor phases
  * A context has several lanes (EG2_HIP_LANES, 1..8, 4 by default): each
  * lane is a stream on a hardware queue of its own (the stream carries a
