@@ -87,8 +87,31 @@ bool valid(const eg2_window_attention_args& a) {
   return need == 0 || (a.workspace && on(a.workspace, 16) && a.workspace_bytes >= need);
 }
 
-template <class Args, class Launch>
-int checked(const Args* args, void* stream, Launch launch) {
+hipError_t launch_linear(const eg2::block::Linear& p, unsigned type, unsigned weight_type, bool gated, hipStream_t st) {
+  switch (type) {
+    case EG2_TYPE_F32:
+      return eg2::block::launch_linear_f32(p, weight_type, gated, st);
+    case EG2_TYPE_F16:
+      return eg2::block::launch_linear_f16(p, weight_type, gated, st);
+    default:
+      return eg2::block::launch_linear_bf16(p, weight_type, gated, st);
+  }
+}
+hipError_t launch(const eg2_linear_args& a, hipStream_t st) {
+  return launch_linear({a.y, a.x, {a.weight, nullptr}, {a.bias, nullptr}, a.residual, a.ldx, a.ldw, a.ldy, a.ldr, a.n, a.k,
+                        a.m, a.act},
+                       a.type, a.weight_type, false, st);
+}
+hipError_t launch(const eg2_linear_gated_args& a, hipStream_t st) {
+  return launch_linear({a.y, a.x, {a.gate, a.up}, {a.gate_bias, a.up_bias}, nullptr, a.ldx, a.ldw, a.ldy, 0, a.n, a.k, a.m,
+                        a.act},
+                       a.type, a.weight_type, true, st);
+}
+hipError_t launch(const eg2_heads_norm_rope_args& a, hipStream_t st) { return eg2::block::launch_heads_norm_rope(a, st); }
+hipError_t launch(const eg2_window_attention_args& a, hipStream_t st) { return eg2::block::launch_window_attention(a, st); }
+
+template <class Args>
+int checked(const Args* args, void* stream) {
   if (!args || !valid(*args)) return kInvalid;
   return (int)launch(*args, reinterpret_cast<hipStream_t>(stream));
 }
@@ -98,19 +121,19 @@ int checked(const Args* args, void* stream, Launch launch) {
 extern "C" {
 
 int eg2_hip_linear(const eg2_linear_args* args, void* stream) {
-  return checked(args, stream, eg2::block::launch_linear);
+  return checked(args, stream);
 }
 
 int eg2_hip_linear_gated(const eg2_linear_gated_args* args, void* stream) {
-  return checked(args, stream, eg2::block::launch_linear_gated);
+  return checked(args, stream);
 }
 
 int eg2_hip_heads_norm_rope(const eg2_heads_norm_rope_args* args, void* stream) {
-  return checked(args, stream, eg2::block::launch_heads_norm_rope);
+  return checked(args, stream);
 }
 
 int eg2_hip_window_attention(const eg2_window_attention_args* args, void* stream) {
-  return checked(args, stream, eg2::block::launch_window_attention);
+  return checked(args, stream);
 }
 
 uint64_t eg2_hip_window_attention_workspace(const eg2_window_attention_args* args) {
