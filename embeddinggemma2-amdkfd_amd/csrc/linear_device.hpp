@@ -19,31 +19,8 @@
 namespace eg2 {
 namespace block {
 
-typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bfloatx8 __attribute__((ext_vector_type(8)));
-
 template <class W>
 constexpr bool kIsQ8 = __is_same(W, Q8);
-// Values in 16 bytes.
-template <class T>
-constexpr int kPer16 = 16 / (int)sizeof(T);
-
-// c += a . b over 16 bytes of each lane: 32 values deep (16-bit types), 16 (fp32).
-template <class T>
-__device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c) {
-  if constexpr (__is_same(T, float)) {
-    const floatx4 fa = __builtin_bit_cast(floatx4, a), fb = __builtin_bit_cast(floatx4, b);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[e], fb[e], c, 0, 0, 0);
-    return c;
-  } else if constexpr (__is_same(T, _Float16)) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0,
-                                                  0);
-  } else {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bfloatx8, a), __builtin_bit_cast(bfloatx8, b), c,
-                                                   0, 0, 0);
-  }
-}
 
 // Loads at any alignment of the values (one instruction: global loads need none).
 template <class V>

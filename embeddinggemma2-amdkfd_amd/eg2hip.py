@@ -12,6 +12,7 @@ no fallback path: a missing library raises immediately.
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libeg2hip.so")
@@ -104,10 +105,23 @@ class EgSaxpy(C.Structure):
 
 # The records of the block operators (include/eg2_hip.h) and the ids of their types and activations.
 _u64 = C.c_uint64
+_torch_types = None  # ops._types()
+
+
+def _packed(cls):
+    """Gives a record class pack(*fields): the record's bytes, in a fraction of the time of its constructor."""
+    codes = {_vp: "P", _u64: "Q", _u: "I", C.c_int: "i", C.c_float: "f"}
+    packer = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0Q")  # 0Q: padded as the record is
+    assert packer.size == C.sizeof(cls)
+    cls.pack = staticmethod(packer.pack)
+    return cls
+
+
 TYPE_F32, TYPE_F16, TYPE_Q8_0, TYPE_BF16 = 0, 1, 8, 30
 ACTIVATIONS = {"none": 0, "gelu": 1, "silu": 2, "relu": 3}
 
 
+@_packed
 class LinearArgs(C.Structure):
     """eg2_linear_args."""
     _fields_ = [("y", _vp), ("x", _vp), ("weight", _vp), ("bias", _vp), ("residual", _vp), ("ldx", _u64),
@@ -115,6 +129,7 @@ class LinearArgs(C.Structure):
                 ("weight_type", _u), ("act", _u)]
 
 
+@_packed
 class LinearGatedArgs(C.Structure):
     """eg2_linear_gated_args."""
     _fields_ = [("y", _vp), ("x", _vp), ("gate", _vp), ("up", _vp), ("gate_bias", _vp), ("up_bias", _vp),
@@ -122,6 +137,7 @@ class LinearGatedArgs(C.Structure):
                 ("weight_type", _u), ("act", _u)]
 
 
+@_packed
 class HeadsNormRopeArgs(C.Structure):
     """eg2_heads_norm_rope_args."""
     _fields_ = [("q_out", _vp), ("k_out", _vp), ("q", _vp), ("k", _vp), ("q_weight", _vp), ("k_weight", _vp),
@@ -131,6 +147,7 @@ class HeadsNormRopeArgs(C.Structure):
                 ("eps", C.c_float), ("q_scale", C.c_float)]
 
 
+@_packed
 class WindowAttentionArgs(C.Structure):
     """eg2_window_attention_args."""
     _fields_ = [("out", _vp), ("q", _vp), ("k", _vp), ("v", _vp), ("q_offsets", _vp), ("k_offsets", _vp),
@@ -169,11 +186,11 @@ SIGNATURES = {
     "eg2_hip_gemm_q8_geglu": (C.c_int, [_vp, _vp, _u, _vp, _vp, _u, _vp, _vp, _u, _u, _u, _u, _vp]),
     "eg2_hip_gemm_q8_qkv_rope": (C.c_int, [_vp, _vp, _u, _vp, _vp, _u, _u, _u, _vp, _vp, _vp, _vp, C.c_float, _vp,
                                            _vp]),
-    "eg2_hip_linear": (C.c_int, [C.POINTER(LinearArgs), _vp]),
-    "eg2_hip_linear_gated": (C.c_int, [C.POINTER(LinearGatedArgs), _vp]),
-    "eg2_hip_heads_norm_rope": (C.c_int, [C.POINTER(HeadsNormRopeArgs), _vp]),
-    "eg2_hip_window_attention": (C.c_int, [C.POINTER(WindowAttentionArgs), _vp]),
-    "eg2_hip_window_attention_workspace": (C.c_uint64, [C.POINTER(WindowAttentionArgs)]),
+    "eg2_hip_linear": (C.c_int, [_vp, _vp]),
+    "eg2_hip_linear_gated": (C.c_int, [_vp, _vp]),
+    "eg2_hip_heads_norm_rope": (C.c_int, [_vp, _vp]),
+    "eg2_hip_window_attention": (C.c_int, [_vp, _vp]),
+    "eg2_hip_window_attention_workspace": (C.c_uint64, [_vp]),
     "eg2_hip_error_string": (C.c_char_p, [C.c_int]),
     "eg2_hip_device_check": (C.c_int, [C.c_char_p, C.c_size_t]),
     "eg2_q8_tile_bytes": (C.c_size_t, [C.c_size_t, _u]),
@@ -784,122 +801,138 @@ class ops:
               "gemm_q8_geglu")
 
     # ---- block operators: any geometry, fp32 / fp16 / bf16 (include/eg2_hip.h). They run on the current
-    # stream of their tensors' device.
+    # stream of their tensors' device. A call's checks and its record are most of a small call's time: sizes, strides
+    # and devices are compared as numbers, and the record is packed in one step.
 
     @staticmethod
-    def _type(t, what):
-        """The id of an activation tensor's type."""
-        import torch
+    def _types():
+        """The ids of the activation types and torch's float32, int32 and uint8."""
+        global _torch_types
+        if _torch_types is None:
+            import torch
 
-        types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-        if t.dtype not in types:
-            raise ValueError(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
-        return types[t.dtype]
-
-    @staticmethod
-    def _on(what, device, **tensors):
-        """Every tensor that is given lies on the GPU `device`."""
-        if device.type != "cuda":
-            raise ValueError(f"{what}: tensors on {device}, not on a GPU")
-        for name, t in tensors.items():
-            if t is not None and t.device != device:
-                raise ValueError(f"{what}: {name} is on {t.device}, not on {device}")
+            _torch_types = ({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16},
+                            torch.float32, torch.int32, torch.uint8)
+        return _torch_types
 
     @staticmethod
-    def _row_stride(t, what, name):
-        """Elements between the rows of a matrix whose rows are dense."""
-        if t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] > 1):
+    def _matrix(t, what, name):
+        """(rows, columns, elements between rows) of a matrix of dense rows."""
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
             raise ValueError(f"{what}: {name} is no matrix of dense rows")
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+        rows, cols = shape
+        return rows, cols, stride[0] if rows > 1 else cols
 
     @staticmethod
-    def _head_strides(t, what, name):
-        """Elements between the rows and the heads of [rows, heads, d] with dense heads."""
-        if t.dim() != 3 or (t.stride(2) != 1 and t.shape[2] > 1):
+    def _heads(t, what, name):
+        """(rows, heads, d, elements between rows, between heads) of [rows, heads, d] with dense heads."""
+        shape, stride = t.shape, t.stride()
+        if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1):
             raise ValueError(f"{what}: {name} is not [rows, heads, d] with dense heads")
-        head = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-        return t.stride(0) if t.shape[0] > 1 else t.shape[1] * head, head
+        rows, heads, d = shape
+        head = stride[1] if heads > 1 else d
+        return rows, heads, d, stride[0] if rows > 1 else heads * head, head
 
     @staticmethod
-    def _vector(t, what, name, n, dtype):
-        """A dense vector of n values of a type, if given."""
-        if t is not None and (t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or not t.is_contiguous()):
+    def _vector(t, what, name, n, dtype, device):
+        """The address of a dense vector of n values of a type on the device; None: 0."""
+        if t is None:
+            return 0
+        if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
             raise ValueError(f"{what}: {name} is not {n} dense values of {dtype}")
+        if t.get_device() != device:
+            raise ValueError(f"{what}: {name} is on another device")
+        return t.data_ptr()
 
-    @classmethod
-    def _launch(cls, what, entry, args, device):
+    @staticmethod
+    def _same_device(what, device, *tensors):
+        for t in tensors:
+            if t.get_device() != device:
+                raise ValueError(f"{what}: tensors on {t.device} and on GPU {device}")
+        if device < 0:
+            raise ValueError(f"{what}: the tensors are not on a GPU")
+
+    @staticmethod
+    def _launch(what, entry, record, device):
         import torch
 
-        if torch.cuda.current_device() == device.index:
-            check(entry(C.byref(args), cls._stream()), what)
+        stream = torch.cuda.current_stream(device).cuda_stream
+        if torch.cuda.current_device() == device:
+            code = entry(record, stream)
         else:
             with torch.cuda.device(device):
-                check(entry(C.byref(args), cls._stream()), what)
+                code = entry(record, stream)
+        if code:
+            check(code, what)
 
     @classmethod
-    def _weights(cls, what, w, name, m, k, x):
+    def _weights(cls, what, w, name, m, k, kind):
         """(type id, row stride in values) of [m, k] weights: uint8 tensors hold rows of Q8_0 blocks."""
-        import torch
-
-        ld = cls._row_stride(w, what, name)
-        if w.dtype == torch.uint8:
-            if k % 32 or tuple(w.shape) != (m, k // 32 * 34) or ld % 34:
+        ids, float32, _, uint8 = cls._types()
+        rows, cols, ld = cls._matrix(w, what, name)
+        if w.dtype == uint8:
+            if k % 32 or rows != m or cols != k // 32 * 34 or ld % 34:
                 raise ValueError(f"{what}: {name} is not {m} rows of {k} Q8_0 values (whole blocks of 34 bytes)")
             return TYPE_Q8_0, ld // 34 * 32
-        if tuple(w.shape) != (m, k):
-            raise ValueError(f"{what}: {name} is {tuple(w.shape)}, not {(m, k)}")
-        if x.dtype != torch.float32 and w.dtype != x.dtype:
-            raise ValueError(f"{what}: {name} of {w.dtype} with activations of {x.dtype}")
-        return cls._type(w, what), ld
+        wtype = ids.get(w.dtype)
+        if rows != m or cols != k or wtype is None or (kind != TYPE_F32 and wtype != kind):
+            raise ValueError(f"{what}: {name} is {tuple(w.shape)} of {w.dtype}: not [{m}, {k}] of a type that fits")
+        return wtype, ld
+
+    @classmethod
+    def _product(cls, what, x, y):
+        """(type id, n, k, m, strides of x and y) of a product's activations and result."""
+        kind = cls._types()[0].get(x.dtype)
+        n, k, ldx = cls._matrix(x, what, "x")
+        rows, m, ldy = cls._matrix(y, what, "y")
+        if kind is None:
+            raise ValueError(f"{what}: x of {x.dtype} is not float32, float16 or bfloat16")
+        if rows != n or y.dtype != x.dtype:
+            raise ValueError(f"{what}: y is {tuple(y.shape)} of {y.dtype}, not {n} rows of {x.dtype}")
+        return kind, n, k, m, ldx, ldy
 
     @classmethod
     def linear(cls, x, weight, y, bias=None, act="none", residual=None):
         """y = act(x . weight^T + bias) + residual (eg2_hip_linear): x [n, k],
         weight [m, k] or uint8 [m, 34 k / 32] of Q8_0 blocks, y [n, m], bias
         float32 [m], residual [n, m] (may be y); act "none", "gelu", "silu" or "relu"."""
-        import torch
-
         what = "linear"
-        kind, ldx, ldy = cls._type(x, what), cls._row_stride(x, what, "x"), cls._row_stride(y, what, "y")
-        (n, k), m = x.shape, y.shape[1]
-        if y.shape[0] != n or y.dtype != x.dtype:
-            raise ValueError(f"{what}: y is {tuple(y.shape)} of {y.dtype}, not {n} rows of {x.dtype}")
-        wtype, ldw = cls._weights(what, weight, "weight", m, k, x)
-        cls._vector(bias, what, "bias", m, torch.float32)
-        ldr = 0
+        kind, n, k, m, ldx, ldy = cls._product(what, x, y)
+        wtype, ldw = cls._weights(what, weight, "weight", m, k, kind)
+        device, res, ldr = x.get_device(), 0, 0
         if residual is not None:
-            ldr = cls._row_stride(residual, what, "residual")
-            if residual.shape != y.shape or residual.dtype != y.dtype:
+            rows, cols, ldr = cls._matrix(residual, what, "residual")
+            if rows != n or cols != m or residual.dtype != x.dtype:
                 raise ValueError(f"{what}: residual is not of y's shape and type")
+            cls._same_device(what, device, residual)
+            res = residual.data_ptr()
         if act not in ACTIVATIONS:
             raise ValueError(f"{what}: no activation {act!r}")
-        cls._on(what, x.device, weight=weight, y=y, bias=bias, residual=residual)
-        args = LinearArgs(cls._p(y), cls._p(x), cls._p(weight), cls._p(bias), cls._p(residual), ldx, ldw, ldy, ldr, n,
-                          k, m, kind, wtype, ACTIVATIONS[act])
-        cls._launch(what, lib().eg2_hip_linear, args, x.device)
+        cls._same_device(what, device, weight, y)
+        record = LinearArgs.pack(y.data_ptr(), x.data_ptr(), weight.data_ptr(),
+                                 cls._vector(bias, what, "bias", m, cls._types()[1], device), res, ldx, ldw, ldy, ldr,
+                                 n, k, m, kind, wtype, ACTIVATIONS[act])
+        cls._launch(what, lib().eg2_hip_linear, record, device)
 
     @classmethod
     def linear_gated(cls, x, gate, up, y, gate_bias=None, up_bias=None, act="gelu"):
         """y = act(x . gate^T + gate_bias) * (x . up^T + up_bias)
         (eg2_hip_linear_gated): the arguments of linear, gate and up alike."""
-        import torch
-
         what = "linear_gated"
-        kind, ldx, ldy = cls._type(x, what), cls._row_stride(x, what, "x"), cls._row_stride(y, what, "y")
-        (n, k), m = x.shape, y.shape[1]
-        if y.shape[0] != n or y.dtype != x.dtype:
-            raise ValueError(f"{what}: y is {tuple(y.shape)} of {y.dtype}, not {n} rows of {x.dtype}")
-        wtype, ldw = cls._weights(what, gate, "gate", m, k, x)
-        if cls._weights(what, up, "up", m, k, x) != (wtype, ldw):
+        kind, n, k, m, ldx, ldy = cls._product(what, x, y)
+        wtype, ldw = cls._weights(what, gate, "gate", m, k, kind)
+        if cls._weights(what, up, "up", m, k, kind) != (wtype, ldw):
             raise ValueError(f"{what}: gate and up differ in type or stride")
-        cls._vector(gate_bias, what, "gate_bias", m, torch.float32)
-        cls._vector(up_bias, what, "up_bias", m, torch.float32)
         if act not in ACTIVATIONS:
             raise ValueError(f"{what}: no activation {act!r}")
-        cls._on(what, x.device, gate=gate, up=up, y=y, gate_bias=gate_bias, up_bias=up_bias)
-        args = LinearGatedArgs(cls._p(y), cls._p(x), cls._p(gate), cls._p(up), cls._p(gate_bias), cls._p(up_bias), ldx,
-                               ldw, ldy, n, k, m, kind, wtype, ACTIVATIONS[act])
-        cls._launch(what, lib().eg2_hip_linear_gated, args, x.device)
+        device, float32 = x.get_device(), cls._types()[1]
+        cls._same_device(what, device, gate, up, y)
+        record = LinearGatedArgs.pack(y.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(),
+                                      cls._vector(gate_bias, what, "gate_bias", m, float32, device),
+                                      cls._vector(up_bias, what, "up_bias", m, float32, device), ldx, ldw, ldy, n, k, m,
+                                      kind, wtype, ACTIVATIONS[act])
+        cls._launch(what, lib().eg2_hip_linear_gated, record, device)
 
     @classmethod
     def heads_norm_rope(cls, q, k, q_w, k_w, table, pos, eps, q_out, k_out, q_scale=1.0):
@@ -908,37 +941,43 @@ class ops:
         rotated by table[pos] (float32 [positions, rotary] as rope_table, int32
         [rows]; both None: not rotated) and, of q, scaled, into q_out and k_out,
         which may be q and k (eg2_hip_heads_norm_rope)."""
-        import torch
-
         what = "heads_norm_rope"
-        rows, heads, d = q.shape if q.dim() == 3 else (0, 0, 0)
-        args = HeadsNormRopeArgs(type=cls._type(q, what), rows=rows, q_heads=heads, d=d, eps=eps, q_scale=q_scale,
-                                 q=cls._p(q), q_out=cls._p(q_out), q_weight=cls._p(q_w))
-        args.q_row, args.q_head = cls._head_strides(q, what, "q")
-        args.q_out_row, args.q_out_head = cls._head_strides(q_out, what, "q_out")
+        ids, float32, int32, _ = cls._types()
+        kind, device = ids.get(q.dtype), q.get_device()
+        if kind is None:
+            raise ValueError(f"{what}: q of {q.dtype} is not float32, float16 or bfloat16")
+        rows, heads, d, q_row, q_head = cls._heads(q, what, "q")
         if q_out.shape != q.shape or q_out.dtype != q.dtype:
             raise ValueError(f"{what}: q_out is not of q's shape and type")
-        cls._vector(q_w, what, "q_w", d, torch.float32)
+        _, _, _, qo_row, qo_head = cls._heads(q_out, what, "q_out")
+        cls._same_device(what, device, q_out)
+        kp = kop = k_heads = k_row = k_head = ko_row = ko_head = 0
         if (k is None) != (k_out is None):
             raise ValueError(f"{what}: k and k_out go together")
         if k is not None:
-            args.k_row, args.k_head = cls._head_strides(k, what, "k")
-            args.k_out_row, args.k_out_head = cls._head_strides(k_out, what, "k_out")
-            if k.shape[0] != rows or k.shape[2] != d or k.dtype != q.dtype:
+            k_rows, k_heads, k_d, k_row, k_head = cls._heads(k, what, "k")
+            if k_rows != rows or k_d != d or k.dtype != q.dtype:
                 raise ValueError(f"{what}: k is {tuple(k.shape)} of {k.dtype}, not {rows} rows of heads of {d}, {q.dtype}")
             if k_out.shape != k.shape or k_out.dtype != k.dtype:
                 raise ValueError(f"{what}: k_out is not of k's shape and type")
-            cls._vector(k_w, what, "k_w", d, torch.float32)
-            args.k_heads, args.k, args.k_out, args.k_weight = k.shape[1], cls._p(k), cls._p(k_out), cls._p(k_w)
+            _, _, _, ko_row, ko_head = cls._heads(k_out, what, "k_out")
+            cls._same_device(what, device, k, k_out)
+            kp, kop = k.data_ptr(), k_out.data_ptr()
         if (table is None) != (pos is None):
             raise ValueError(f"{what}: table and pos go together")
+        tp = positions = rotary = 0
         if table is not None:
-            if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+            if len(table.shape) != 2 or table.dtype != float32 or not table.is_contiguous():
                 raise ValueError(f"{what}: table is not a dense float32 matrix")
-            cls._vector(pos, what, "pos", rows, torch.int32)
-            args.table, args.pos, args.table_rows, args.rotary = cls._p(table), cls._p(pos), *table.shape
-        cls._on(what, q.device, k=k, q_w=q_w, k_w=k_w, table=table, pos=pos, q_out=q_out, k_out=k_out)
-        cls._launch(what, lib().eg2_hip_heads_norm_rope, args, q.device)
+            (positions, rotary), tp = table.shape, table.data_ptr()
+            cls._same_device(what, device, table)
+        record = HeadsNormRopeArgs.pack(q_out.data_ptr(), kop, q.data_ptr(), kp,
+                                        cls._vector(q_w, what, "q_w", d, float32, device),
+                                        cls._vector(k_w, what, "k_w", d, float32, device), tp,
+                                        cls._vector(pos, what, "pos", rows, int32, device), q_row, q_head, k_row, k_head,
+                                        qo_row, qo_head, ko_row, ko_head, rows, heads, k_heads, d, rotary, positions,
+                                        kind, eps, q_scale)
+        cls._launch(what, lib().eg2_hip_heads_norm_rope, record, device)
 
     @classmethod
     def window_attention(cls, q, k, v, q_offsets, k_offsets, out, scale, left=-1, right=-1, sinks=0, k_lengths=None,
@@ -949,43 +988,48 @@ class ops:
         and the first `sinks` (eg2_hip_window_attention). longest: the longest
         sequence of keys, a hint. workspace: a uint8 tensor of
         window_attention_workspace's bytes; by default one is taken from torch."""
-        import torch
-
         what = "window_attention"
-        if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or out.shape != q.shape or k.shape[2] != q.shape[2]:
+        ids, _, int32, uint8 = cls._types()
+        kind, device = ids.get(q.dtype), q.get_device()
+        rows, heads, d, q_row, q_head = cls._heads(q, what, "q")
+        key_rows, kv_heads, k_d, k_row, k_head = cls._heads(k, what, "k")
+        if kind is None or not q.dtype == k.dtype == v.dtype == out.dtype:
+            raise ValueError(f"{what}: q, k, v and out are not all float32, float16 or bfloat16")
+        if k_d != d or v.shape != k.shape or out.shape != q.shape:
             raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and out "
                              f"{tuple(out.shape)} do not fit")
-        if not q.dtype == k.dtype == v.dtype == out.dtype:
-            raise ValueError(f"{what}: q, k, v and out differ in type")
+        _, _, _, v_row, v_head = cls._heads(v, what, "v")
+        _, _, _, out_row, out_head = cls._heads(out, what, "out")
         batch = q_offsets.numel() - 1
-        for name, t, n in (("q_offsets", q_offsets, batch + 1), ("k_offsets", k_offsets, batch + 1),
-                           ("k_lengths", k_lengths, batch)):
-            cls._vector(t, what, name, n, torch.int32)
-        cls._on(what, q.device, k=k, v=v, out=out, q_offsets=q_offsets, k_offsets=k_offsets, k_lengths=k_lengths,
-                workspace=workspace)
-        args = WindowAttentionArgs(cls._p(out), cls._p(q), cls._p(k), cls._p(v), cls._p(q_offsets), cls._p(k_offsets),
-                                   cls._p(k_lengths), None, 0, *cls._head_strides(q, what, "q"),
-                                   *cls._head_strides(k, what, "k"), *cls._head_strides(v, what, "v"),
-                                   *cls._head_strides(out, what, "out"), max(batch, 0), q.shape[0], k.shape[0],
-                                   q.shape[1], k.shape[1], q.shape[2], cls._type(q, what), left, right, sinks, longest,
-                                   scale)
-        need = lib().eg2_hip_window_attention_workspace(C.byref(args))
-        if workspace is None and need:  # torch keeps it for this stream until the kernels are done
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        if batch < 0:
+            raise ValueError(f"{what}: no offsets")
+        cls._same_device(what, device, k, v, out)
+        offsets = (cls._vector(q_offsets, what, "q_offsets", batch + 1, int32, device),
+                   cls._vector(k_offsets, what, "k_offsets", batch + 1, int32, device),
+                   cls._vector(k_lengths, what, "k_lengths", batch, int32, device))
+        sizes = (batch, rows, key_rows, heads, kv_heads, d, kind, left, right, sinks, longest, scale)
+        strides = (q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head)
+        pointers = (out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *offsets)
+        space, need = 0, 0
+        if workspace is None:
+            need = lib().eg2_hip_window_attention_workspace(WindowAttentionArgs.pack(*pointers, 0, 0, *strides, *sizes))
+            if need:  # torch keeps it for this stream until the kernels are done
+                import torch
+
+                workspace = torch.empty(need, dtype=uint8, device=q.device)
         if workspace is not None:
-            if workspace.dtype != torch.uint8 or not workspace.is_contiguous():
-                raise ValueError(f"{what}: workspace is not a dense uint8 tensor")
-            args.workspace, args.workspace_bytes = cls._p(workspace), workspace.numel()
-        cls._launch(what, lib().eg2_hip_window_attention, args, q.device)
+            need = workspace.numel()
+            space = cls._vector(workspace, what, "workspace", need, uint8, device)
+        record = WindowAttentionArgs.pack(*pointers, space, need, *strides, *sizes)
+        cls._launch(what, lib().eg2_hip_window_attention, record, device)
 
     @classmethod
     def window_attention_workspace(cls, batch, rows, key_rows, heads, kv_heads, d, dtype, left=-1, right=-1, sinks=0,
                                    longest=0):
         """Bytes of workspace of a window_attention call of these sizes."""
-        import torch
-
-        types = {torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16}
-        args = WindowAttentionArgs(batch=batch, rows=rows, key_rows=key_rows, heads=heads, kv_heads=kv_heads, d=d,
-                                   type=types.get(dtype, 0xffffffff), left=left, right=right, sinks=sinks,
-                                   longest=longest)
-        return lib().eg2_hip_window_attention_workspace(C.byref(args))
+        kind = cls._types()[0].get(dtype)
+        if kind is None:
+            raise ValueError(f"window_attention_workspace: {dtype} is not float32, float16 or bfloat16")
+        return lib().eg2_hip_window_attention_workspace(
+            WindowAttentionArgs.pack(*(0,) * 9, *(0,) * 8, batch, rows, key_rows, heads, kv_heads, d, kind, left, right,
+                                     sinks, longest, 1.0))

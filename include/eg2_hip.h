@@ -313,7 +313,7 @@ int eg2_hip_heads_norm_rope(const eg2_heads_norm_rope_args *args, void *stream);
  * and v that may be touched. q, k, v and out are of `type`, F32, F16 or BF16;
  * d: a multiple of 8, 8 to 256; their pointers lie on 16 bytes and their strides are
  * multiples of 16 bytes. heads is a multiple of kv_heads, at most 4096. batch: 1 to 65535;
- * rows and key_rows: 1 to 2^31 - 1. longest: the longest
+ * rows and key_rows: 1 to 2^31 - 1; rows heads at most 2^27, batch kv_heads 2^22. longest: the longest
  * sequence of keys (0: unknown), a hint: it chooses how the keys of few queries are
  * split over the GPU, which costs time or the order of sums, never a key. workspace: device memory of
  * at least eg2_hip_window_attention_workspace(args) bytes (which may be 0), 16-byte
