@@ -68,6 +68,11 @@ __device__ __forceinline__ floatx4 mfma16(uintx4 a, uintx4 b, floatx4 c) {
   }
 }
 
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
 // Calls f with a value of the C++ type of an EG2_TYPE_ id of activations.
 template <class F>
 auto with_type(unsigned type, F f) {

@@ -32,10 +32,6 @@ namespace {
 
 typedef eg2_window_attention_args Args;
 typedef short shortx4 __attribute__((ext_vector_type(4)));
-template <int N>
-struct Const {
-  static constexpr int value = N;
-};
 
 struct Sequence {
   int q0, k0;  // first rows
