@@ -801,137 +801,107 @@ class ops:
               "gemm_q8_geglu")
 
     # ---- block operators: any geometry, fp32 / fp16 / bf16 (include/eg2_hip.h). They run on the current
-    # stream of their tensors' device. A call's checks and its record are most of a small call's time: sizes, strides
-    # and devices are compared as numbers, and the record is packed in one step.
+    # stream of their tensors' device. A call's checks and its record are most of a small call's time: all that must hold
+    # is one condition, and what is wrong is looked for only when something is.
 
     @staticmethod
     def _types():
-        """The ids of the activation types and torch's float32, int32 and uint8."""
+        """(ids of the activation types, torch's float32, int32, uint8, the current raw stream of a device, torch.cuda)."""
         global _torch_types
         if _torch_types is None:
             import torch
 
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # the number alone, without its object
             _torch_types = ({torch.float32: TYPE_F32, torch.float16: TYPE_F16, torch.bfloat16: TYPE_BF16},
-                            torch.float32, torch.int32, torch.uint8)
+                            torch.float32, torch.int32, torch.uint8,
+                            raw or (lambda device: torch.cuda.current_stream(device).cuda_stream), torch.cuda)
         return _torch_types
 
     @staticmethod
-    def _matrix(t, what, name):
-        """(rows, columns, elements between rows) of a matrix of dense rows."""
-        shape, stride = t.shape, t.stride()
-        if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
-            raise ValueError(f"{what}: {name} is no matrix of dense rows")
-        rows, cols = shape
-        return rows, cols, stride[0] if rows > 1 else cols
+    def _refuse(what, **tensors):
+        """Raises for tensors that do not fit together."""
+        said = ", ".join(f"{name} {tuple(t.shape)} strides {t.stride()} {t.dtype} on {t.device}"
+                         for name, t in tensors.items() if t is not None)
+        raise ValueError(f"{what}: not tensors of one GPU whose sizes and types fit, with dense last dimensions: {said}")
 
-    @staticmethod
-    def _heads(t, what, name):
-        """(rows, heads, d, elements between rows, between heads) of [rows, heads, d] with dense heads."""
-        shape, stride = t.shape, t.stride()
-        if len(shape) != 3 or (stride[2] != 1 and shape[2] > 1):
-            raise ValueError(f"{what}: {name} is not [rows, heads, d] with dense heads")
-        rows, heads, d = shape
-        head = stride[1] if heads > 1 else d
-        return rows, heads, d, stride[0] if rows > 1 else heads * head, head
-
-    @staticmethod
-    def _vector(t, what, name, n, dtype, device):
+    @classmethod
+    def _vector(cls, t, what, name, n, dtype, device):
         """The address of a dense vector of n values of a type on the device; None: 0."""
         if t is None:
             return 0
-        if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
-            raise ValueError(f"{what}: {name} is not {n} dense values of {dtype}")
-        if t.get_device() != device:
-            raise ValueError(f"{what}: {name} is on another device")
+        if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous() or t.get_device() != device:
+            raise ValueError(f"{what}: {name} is not {n} dense values of {dtype} on the same GPU: {tuple(t.shape)} {t.dtype} "
+                             f"on {t.device}")
         return t.data_ptr()
 
     @staticmethod
-    def _same_device(what, device, *tensors):
-        for t in tensors:
-            if t.get_device() != device:
-                raise ValueError(f"{what}: tensors on {t.device} and on GPU {device}")
-        if device < 0:
-            raise ValueError(f"{what}: the tensors are not on a GPU")
-
-    @staticmethod
     def _launch(what, entry, record, device):
-        import torch
-
-        stream = torch.cuda.current_stream(device).cuda_stream
-        if torch.cuda.current_device() == device:
+        _, _, _, _, stream_of, cuda = _torch_types
+        stream = stream_of(device)
+        if cuda.current_device() == device:
             code = entry(record, stream)
         else:
-            with torch.cuda.device(device):
+            with cuda.device(device):
                 code = entry(record, stream)
         if code:
             check(code, what)
 
     @classmethod
-    def _weights(cls, what, w, name, m, k, kind):
-        """(type id, row stride in values) of [m, k] weights: uint8 tensors hold rows of Q8_0 blocks."""
-        ids, float32, _, uint8 = cls._types()
-        rows, cols, ld = cls._matrix(w, what, name)
-        if w.dtype == uint8:
-            if k % 32 or rows != m or cols != k // 32 * 34 or ld % 34:
-                raise ValueError(f"{what}: {name} is not {m} rows of {k} Q8_0 values (whole blocks of 34 bytes)")
-            return TYPE_Q8_0, ld // 34 * 32
-        wtype = ids.get(w.dtype)
-        if rows != m or cols != k or wtype is None or (kind != TYPE_F32 and wtype != kind):
-            raise ValueError(f"{what}: {name} is {tuple(w.shape)} of {w.dtype}: not [{m}, {k}] of a type that fits")
-        return wtype, ld
-
-    @classmethod
-    def _product(cls, what, x, y):
-        """(type id, n, k, m, strides of x and y) of a product's activations and result."""
-        kind = cls._types()[0].get(x.dtype)
-        n, k, ldx = cls._matrix(x, what, "x")
-        rows, m, ldy = cls._matrix(y, what, "y")
-        if kind is None:
-            raise ValueError(f"{what}: x of {x.dtype} is not float32, float16 or bfloat16")
-        if rows != n or y.dtype != x.dtype:
-            raise ValueError(f"{what}: y is {tuple(y.shape)} of {y.dtype}, not {n} rows of {x.dtype}")
-        return kind, n, k, m, ldx, ldy
+    def _product(cls, what, x, w, y, act):
+        """(n, k, m, type id, type id and strides of the weights, strides of x and y, activation id, GPU)."""
+        ids, _, _, uint8, _, _ = _torch_types or cls._types()
+        act_id = ACTIVATIONS.get(act)
+        if act_id is None:
+            raise ValueError(f"{what}: no activation {act!r}")
+        if not x.dim() == w.dim() == y.dim() == 2:
+            cls._refuse(what, x=x, weight=w, y=y)
+        (n, k), (ldx, x1), (wm, wk), (ldw, w1) = x.shape, x.stride(), w.shape, w.stride()
+        (rows, m), (ldy, y1) = y.shape, y.stride()
+        dtype, device = x.dtype, x.get_device()
+        kind, wkind = ids.get(dtype), ids.get(w.dtype)
+        if w.dtype is uint8:  # rows of Q8_0 blocks, 34 bytes for 32 values
+            wkind, dense = TYPE_Q8_0, k % 32 == 0 and wk == k // 32 * 34 and (wm == 1 or ldw % 34 == 0)
+            ldw = ldw // 34 * 32
+        else:
+            dense = wk == k and (kind == TYPE_F32 or wkind == kind)
+        if (kind is None or wkind is None or not dense or rows != n or wm != m or y.dtype is not dtype or
+                (x1 != 1 and k > 1) or (w1 != 1 and wk > 1) or (y1 != 1 and m > 1) or
+                not y.get_device() == w.get_device() == device or device < 0):
+            cls._refuse(what, x=x, weight=w, y=y)
+        return (n, k, m, kind, wkind, ldx if n > 1 else k, ldw if m > 1 else k, ldy if n > 1 else m, act_id, device)
 
     @classmethod
     def linear(cls, x, weight, y, bias=None, act="none", residual=None):
         """y = act(x . weight^T + bias) + residual (eg2_hip_linear): x [n, k],
         weight [m, k] or uint8 [m, 34 k / 32] of Q8_0 blocks, y [n, m], bias
         float32 [m], residual [n, m] (may be y); act "none", "gelu", "silu" or "relu"."""
-        what = "linear"
-        kind, n, k, m, ldx, ldy = cls._product(what, x, y)
-        wtype, ldw = cls._weights(what, weight, "weight", m, k, kind)
-        device, res, ldr = x.get_device(), 0, 0
+        n, k, m, kind, wkind, ldx, ldw, ldy, act, device = cls._product("linear", x, weight, y, act)
+        res = ldr = 0
         if residual is not None:
-            rows, cols, ldr = cls._matrix(residual, what, "residual")
-            if rows != n or cols != m or residual.dtype != x.dtype:
-                raise ValueError(f"{what}: residual is not of y's shape and type")
-            cls._same_device(what, device, residual)
-            res = residual.data_ptr()
-        if act not in ACTIVATIONS:
-            raise ValueError(f"{what}: no activation {act!r}")
-        cls._same_device(what, device, weight, y)
-        record = LinearArgs.pack(y.data_ptr(), x.data_ptr(), weight.data_ptr(),
-                                 cls._vector(bias, what, "bias", m, cls._types()[1], device), res, ldx, ldw, ldy, ldr,
-                                 n, k, m, kind, wtype, ACTIVATIONS[act])
-        cls._launch(what, lib().eg2_hip_linear, record, device)
+            if (residual.shape != y.shape or residual.dtype is not y.dtype or residual.get_device() != device or
+                    (residual.stride(1) != 1 and m > 1)):
+                cls._refuse("linear", y=y, residual=residual)
+            res, ldr = residual.data_ptr(), residual.stride(0) if n > 1 else m
+        if bias is not None:
+            bias = cls._vector(bias, "linear", "bias", m, _torch_types[1], device)
+        record = LinearArgs.pack(y.data_ptr(), x.data_ptr(), weight.data_ptr(), bias or 0, res, ldx, ldw, ldy, ldr, n, k,
+                                 m, kind, wkind, act)
+        cls._launch("linear", lib().eg2_hip_linear, record, device)
 
     @classmethod
     def linear_gated(cls, x, gate, up, y, gate_bias=None, up_bias=None, act="gelu"):
         """y = act(x . gate^T + gate_bias) * (x . up^T + up_bias)
         (eg2_hip_linear_gated): the arguments of linear, gate and up alike."""
         what = "linear_gated"
-        kind, n, k, m, ldx, ldy = cls._product(what, x, y)
-        wtype, ldw = cls._weights(what, gate, "gate", m, k, kind)
-        if cls._weights(what, up, "up", m, k, kind) != (wtype, ldw):
-            raise ValueError(f"{what}: gate and up differ in type or stride")
-        if act not in ACTIVATIONS:
-            raise ValueError(f"{what}: no activation {act!r}")
-        device, float32 = x.get_device(), cls._types()[1]
-        cls._same_device(what, device, gate, up, y)
+        n, k, m, kind, wkind, ldx, ldw, ldy, act, device = cls._product(what, x, gate, y, act)
+        if (up.shape != gate.shape or up.stride() != gate.stride() or up.dtype is not gate.dtype or
+                up.get_device() != device):
+            cls._refuse(what, gate=gate, up=up)
+        float32 = _torch_types[1]
         record = LinearGatedArgs.pack(y.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr(),
                                       cls._vector(gate_bias, what, "gate_bias", m, float32, device),
                                       cls._vector(up_bias, what, "up_bias", m, float32, device), ldx, ldw, ldy, n, k, m,
-                                      kind, wtype, ACTIVATIONS[act])
+                                      kind, wkind, act)
         cls._launch(what, lib().eg2_hip_linear_gated, record, device)
 
     @classmethod
@@ -942,41 +912,39 @@ class ops:
         [rows]; both None: not rotated) and, of q, scaled, into q_out and k_out,
         which may be q and k (eg2_hip_heads_norm_rope)."""
         what = "heads_norm_rope"
-        ids, float32, int32, _ = cls._types()
-        kind, device = ids.get(q.dtype), q.get_device()
-        if kind is None:
-            raise ValueError(f"{what}: q of {q.dtype} is not float32, float16 or bfloat16")
-        rows, heads, d, q_row, q_head = cls._heads(q, what, "q")
-        if q_out.shape != q.shape or q_out.dtype != q.dtype:
-            raise ValueError(f"{what}: q_out is not of q's shape and type")
-        _, _, _, qo_row, qo_head = cls._heads(q_out, what, "q_out")
-        cls._same_device(what, device, q_out)
+        ids, float32, int32, _, _, _ = _torch_types or cls._types()
+        if q.dim() != 3 or q_out.dim() != 3:
+            cls._refuse(what, q=q, q_out=q_out)
+        dtype, device, shape = q.dtype, q.get_device(), q.shape
+        kind = ids.get(dtype)
+        (rows, heads, d), (q_row, q_head, q1), (qo_row, qo_head, qo1) = shape, q.stride(), q_out.stride()
+        if (kind is None or q_out.shape != shape or q_out.dtype is not dtype or ((q1 != 1 or qo1 != 1) and d > 1) or
+                q_out.get_device() != device or device < 0):
+            cls._refuse(what, q=q, q_out=q_out)
         kp = kop = k_heads = k_row = k_head = ko_row = ko_head = 0
         if (k is None) != (k_out is None):
             raise ValueError(f"{what}: k and k_out go together")
         if k is not None:
-            k_rows, k_heads, k_d, k_row, k_head = cls._heads(k, what, "k")
-            if k_rows != rows or k_d != d or k.dtype != q.dtype:
-                raise ValueError(f"{what}: k is {tuple(k.shape)} of {k.dtype}, not {rows} rows of heads of {d}, {q.dtype}")
-            if k_out.shape != k.shape or k_out.dtype != k.dtype:
-                raise ValueError(f"{what}: k_out is not of k's shape and type")
-            _, _, _, ko_row, ko_head = cls._heads(k_out, what, "k_out")
-            cls._same_device(what, device, k, k_out)
+            if k.dim() != 3 or k_out.dim() != 3:
+                cls._refuse(what, k=k, k_out=k_out)
+            (k_rows, k_heads, k_d), (k_row, k_head, k1), (ko_row, ko_head, ko1) = k.shape, k.stride(), k_out.stride()
+            if (k_rows != rows or k_d != d or k_out.shape != k.shape or not k.dtype is k_out.dtype is dtype or
+                    ((k1 != 1 or ko1 != 1) and d > 1) or not k.get_device() == k_out.get_device() == device):
+                cls._refuse(what, q=q, k=k, k_out=k_out)
             kp, kop = k.data_ptr(), k_out.data_ptr()
         if (table is None) != (pos is None):
             raise ValueError(f"{what}: table and pos go together")
-        tp = positions = rotary = 0
+        tp = at = positions = rotary = 0
         if table is not None:
-            if len(table.shape) != 2 or table.dtype != float32 or not table.is_contiguous():
-                raise ValueError(f"{what}: table is not a dense float32 matrix")
+            if table.dim() != 2 or table.dtype is not float32 or not table.is_contiguous() or table.get_device() != device:
+                cls._refuse(what, q=q, table=table)
             (positions, rotary), tp = table.shape, table.data_ptr()
-            cls._same_device(what, device, table)
+            at = cls._vector(pos, what, "pos", rows, int32, device)
         record = HeadsNormRopeArgs.pack(q_out.data_ptr(), kop, q.data_ptr(), kp,
                                         cls._vector(q_w, what, "q_w", d, float32, device),
-                                        cls._vector(k_w, what, "k_w", d, float32, device), tp,
-                                        cls._vector(pos, what, "pos", rows, int32, device), q_row, q_head, k_row, k_head,
-                                        qo_row, qo_head, ko_row, ko_head, rows, heads, k_heads, d, rotary, positions,
-                                        kind, eps, q_scale)
+                                        cls._vector(k_w, what, "k_w", d, float32, device), tp, at, q_row, q_head, k_row,
+                                        k_head, qo_row, qo_head, ko_row, ko_head, rows, heads, k_heads, d, rotary,
+                                        positions, kind, eps, q_scale)
         cls._launch(what, lib().eg2_hip_heads_norm_rope, record, device)
 
     @classmethod
@@ -989,38 +957,46 @@ class ops:
         sequence of keys, a hint. workspace: a uint8 tensor of
         window_attention_workspace's bytes; by default one is taken from torch."""
         what = "window_attention"
-        ids, _, int32, uint8 = cls._types()
-        kind, device = ids.get(q.dtype), q.get_device()
-        rows, heads, d, q_row, q_head = cls._heads(q, what, "q")
-        key_rows, kv_heads, k_d, k_row, k_head = cls._heads(k, what, "k")
-        if kind is None or not q.dtype == k.dtype == v.dtype == out.dtype:
-            raise ValueError(f"{what}: q, k, v and out are not all float32, float16 or bfloat16")
-        if k_d != d or v.shape != k.shape or out.shape != q.shape:
-            raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} and out "
-                             f"{tuple(out.shape)} do not fit")
-        _, _, _, v_row, v_head = cls._heads(v, what, "v")
-        _, _, _, out_row, out_head = cls._heads(out, what, "out")
+        ids, _, int32, uint8, _, _ = _torch_types or cls._types()
+        if not q.dim() == k.dim() == v.dim() == out.dim() == 3:
+            cls._refuse(what, q=q, k=k, v=v, out=out)
+        dtype, device, shape, k_shape = q.dtype, q.get_device(), q.shape, k.shape
+        kind = ids.get(dtype)
+        (rows, heads, d), (key_rows, kv_heads, k_d) = shape, k_shape
+        (q_row, q_head, q1), (k_row, k_head, k1) = q.stride(), k.stride()
+        (v_row, v_head, v1), (out_row, out_head, out1) = v.stride(), out.stride()
+        if (kind is None or k_d != d or v.shape != k_shape or out.shape != shape or
+                not k.dtype is v.dtype is out.dtype is dtype or not q1 == k1 == v1 == out1 == 1 or
+                not k.get_device() == v.get_device() == out.get_device() == device or device < 0):
+            cls._refuse(what, q=q, k=k, v=v, out=out)
+        if heads == 1:  # the strides of a dimension of one are anything
+            q_head, out_head = d, d
+        if kv_heads == 1:
+            k_head, v_head = d, d
+        if rows == 1:
+            q_row, out_row = heads * d, heads * d
+        if key_rows == 1:
+            k_row, v_row = kv_heads * d, kv_heads * d
         batch = q_offsets.numel() - 1
         if batch < 0:
             raise ValueError(f"{what}: no offsets")
-        cls._same_device(what, device, k, v, out)
-        offsets = (cls._vector(q_offsets, what, "q_offsets", batch + 1, int32, device),
-                   cls._vector(k_offsets, what, "k_offsets", batch + 1, int32, device),
-                   cls._vector(k_lengths, what, "k_lengths", batch, int32, device))
-        sizes = (batch, rows, key_rows, heads, kv_heads, d, kind, left, right, sinks, longest, scale)
-        strides = (q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head)
-        pointers = (out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *offsets)
-        space, need = 0, 0
+        qo = cls._vector(q_offsets, what, "q_offsets", batch + 1, int32, device)
+        ko = qo if k_offsets is q_offsets else cls._vector(k_offsets, what, "k_offsets", batch + 1, int32, device)
+        kl = 0 if k_lengths is None else cls._vector(k_lengths, what, "k_lengths", batch, int32, device)
+        fields = [out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), qo, ko, kl, 0, 0, q_row, q_head, k_row, k_head,
+                  v_row, v_head, out_row, out_head, batch, rows, key_rows, heads, kv_heads, d, kind, left, right, sinks,
+                  longest, scale]
+        record = WindowAttentionArgs.pack(*fields)
         if workspace is None:
-            need = lib().eg2_hip_window_attention_workspace(WindowAttentionArgs.pack(*pointers, 0, 0, *strides, *sizes))
+            need = lib().eg2_hip_window_attention_workspace(record)
             if need:  # torch keeps it for this stream until the kernels are done
                 import torch
 
                 workspace = torch.empty(need, dtype=uint8, device=q.device)
         if workspace is not None:
-            need = workspace.numel()
-            space = cls._vector(workspace, what, "workspace", need, uint8, device)
-        record = WindowAttentionArgs.pack(*pointers, space, need, *strides, *sizes)
+            fields[8] = workspace.numel()
+            fields[7] = cls._vector(workspace, what, "workspace", fields[8], uint8, device)
+            record = WindowAttentionArgs.pack(*fields)
         cls._launch(what, lib().eg2_hip_window_attention, record, device)
 
     @classmethod
