@@ -13,6 +13,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cstdlib>
 #include "block_device.hpp"
 #include "eg2_block.hpp"
 
@@ -47,8 +48,9 @@ __device__ __forceinline__ uintx4 load_chunk(const W* row, unsigned k, unsigned 
 #pragma unroll
     for (int e = 0; e < N; ++e) r.v[e] = (T)to_float(w.v[e]);
   } else {
+    // The value itself or, past the end, the last one, not used: no branch per value.
 #pragma unroll
-    for (int e = 0; e < N; ++e) r.v[e] = k + e < end ? (T)to_float(row[k + e]) : (T)0.0f;
+    for (int e = 0; e < N; ++e) r.v[e] = k + e < end ? (T)to_float(row[min(k + e, end - 1)]) : (T)0.0f;
   }
   return r.all;
 }
@@ -91,13 +93,50 @@ __device__ __forceinline__ void finish(const Linear& p, unsigned row, unsigned c
   }
 }
 
+// A piece of a Q8_0 block on its way: N values from value `at` (a multiple of N) on,
+// N / 4 + 1 aligned words from byte `at` of the block, rounded down to 4, on. The
+// block lies on 2 bytes: `odd` is at 2 mod 4. Then the values are the words but the
+// first, else they start 2 bytes in; the first word also holds the scale if at is 0.
+// (Loads that are not on 4 bytes take several times as long: 64 cycles each in the
+// few-row form.) The first word may begin 2 bytes before the block, the last
+// end 2 behind it; with `edge` (a matrix's first or last row) no byte
+// outside the block is read.
+template <int N>
+struct Q8Piece {
+  uint32_t w[N / 4 + 1];
+  bool odd;
+  __device__ __forceinline__ void load(const unsigned char* block, unsigned at, bool edge) {
+    odd = (reinterpret_cast<uintptr_t>(block) & 2) != 0;
+    const unsigned char* from = block + at - (odd ? 2 : 0);
+    if (!edge) {
+#pragma unroll
+      for (int i = 0; i <= N / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(from)[i];
+    } else {  // the half word at one end alone
+      const uint32_t half = *reinterpret_cast<const uint16_t*>(block + at + (odd ? 0 : N));
+      const uint32_t* words = reinterpret_cast<const uint32_t*>(from) + (odd ? 1 : 0);
+      uint32_t v[N / 4];
+#pragma unroll
+      for (int i = 0; i < N / 4; ++i) v[i] = words[i];
+#pragma unroll
+      for (int i = 0; i <= N / 4; ++i) w[i] = odd ? (i == 0 ? half << 16 : v[i == 0 ? 0 : i - 1]) : (i == N / 4 ? half : v[i == N / 4 ? 0 : i]);
+    }
+  }
+  __device__ __forceinline__ float scale() const { return fp16_bits_to_fp32(odd ? w[0] >> 16 : w[0] & 0xffffu); }
+  __device__ __forceinline__ float value(int e) const {
+    const uint32_t four = odd ? w[e / 4 + 1] : __builtin_amdgcn_alignbyte(w[e / 4 + 1], w[e / 4], 2);
+    return (float)(int8_t)(four >> (8 * (e % 4)));
+  }
+};
+
 // ------------------------------------------------------------------ tiles
 //
 // BM rows of x times BN rows of the weights (of a gated pair BN / 2 of each
-// matrix) per workgroup of four waves, 2 x 2, each 16 x 16 blocks over its
-// quarter. Slices of 128 bytes of every row go through two LDS buffers, the next
-// on its way while one is multiplied. The 16-byte chunks of a row are
-// swizzled so that the 16 rows of a fragment read lie on distinct banks.
+// matrix) per workgroup of WM x WN waves, each 16 x 16 blocks over its
+// part. Slices of 128 bytes of every row go through NBUF LDS buffers, all but one
+// on their way while one is multiplied. The 16-byte chunks of a row are
+// swizzled so that the 16 rows of a fragment read lie on distinct banks. Rows on
+// 4 bytes go straight to LDS (DMA), others and what has to be decoded through
+// registers.
 constexpr int kRowBytes = 128, kChunks = kRowBytes / 16;
 
 // A wave's block j of JBG, lane i: which of its 16 JBG weight rows it feeds, so
@@ -111,28 +150,24 @@ __device__ __forceinline__ int weight_key(int row) {
   return (row & 3) | ((row / (4 * JBG)) & 1) << 2;
 }
 
-// One Q8_0 item: 16 values of a row and the scale of their block.
-struct Q8Item {
-  uint32_t q[4];
-  uint32_t d;
-};
-
-template <class T, class W, bool GATED, bool DMA, int BM, int BN>
-__global__ void __launch_bounds__(256) linear_tile_kernel(Linear p) {
+template <class T, class W, bool GATED, bool DMA, int BM, int BN, int WM, int WN, int NBUF>
+__global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(Linear p) {
   constexpr int G = GATED ? 2 : 1, COLS = BN / G;  // columns of y
-  constexpr int IB = BM / 32, JB = BN / 32, JBG = JB / G;
+  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  constexpr int IB = BM / 16 / WM, JB = BN / 16 / WN, JBG = JB / G;
   constexpr int N = kPer16<T>, BK = kChunks * N;  // values per chunk and slice
   constexpr bool kScaled = kIsQ8<W> && !__is_same(T, float);
   constexpr bool kDmaW = DMA && __is_same(T, W);
   constexpr int kBlocks = BK / 32;  // Q8_0 blocks of a slice
+  static_assert(NBUF == 2 || kDmaW, "registers hold one slice");
   struct Lds {
-    alignas(16) unsigned char x[2][BM * kRowBytes];
-    alignas(16) unsigned char w[2][BN * kRowBytes];
-    alignas(16) float d[2][kScaled ? kBlocks * BN : 4];
+    alignas(16) unsigned char x[NBUF][BM * kRowBytes];
+    alignas(16) unsigned char w[NBUF][BN * kRowBytes];
+    alignas(16) float d[kScaled ? 2 : 1][kScaled ? kBlocks * BN : 4];
   };
   __shared__ Lds lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, r = lane & 15, wm = wave >> 1, wn = wave & 1;
+  const int g = lane >> 4, r = lane & 15, wm = wave / WN, wn = wave % WN;
 
   // Workgroups go round the 8 XCDs; each XCD takes a run of tiles, eight rows
   // of tiles down before the next column, so that its L2 serves both operands.
@@ -154,36 +189,37 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(Linear p) {
   const T* xrows = static_cast<const T*>(p.x);
 
   // A slice on its way through registers.
-  constexpr int kXItems = BM * kChunks / 256;
-  constexpr int kWItems = kIsQ8<W> ? (BN * BK / 16 + 255) / 256 : BN * kChunks / 256;
-  uintx4 xv[kXItems], wv[kIsQ8<W> ? 1 : kWItems];
-  Q8Item qv[kIsQ8<W> ? kWItems : 1];
+  constexpr int kXItems = BM * kChunks / THREADS;
+  constexpr int kWItems = kIsQ8<W> ? (BN * BK / 16 + THREADS - 1) / THREADS : BN * kChunks / THREADS;
+  uintx4 xv[DMA ? 1 : kXItems], wv[kIsQ8<W> || kDmaW ? 1 : kWItems];
+  Q8Piece<16> qv[kIsQ8<W> ? kWItems : 1];
+  uint32_t qd[kIsQ8<W> && !kScaled ? kWItems : 1];
+  const bool edge = col0 == 0 || col0 + COLS >= p.m;
   auto load = [&](unsigned k0) {
     if constexpr (!DMA) {
 #pragma unroll
       for (int i = 0; i < kXItems; ++i) {
-        const int item = tid + 256 * i, rr = item / kChunks, c = item % kChunks;
+        const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
         xv[i] = load_chunk<T, T>(xrows + min(row0 + rr, p.n - 1) * p.ldx, k0 + N * c, p.k);
       }
     }
     if constexpr (kIsQ8<W>) {
 #pragma unroll
       for (int i = 0; i < kWItems; ++i) {
-        const int item = tid + 256 * i, rr = item / (BK / 16), part = item % (BK / 16);
+        const int item = tid + THREADS * i, rr = item / (BK / 16), part = item % (BK / 16);
         const unsigned k = k0 + 16 * part;
-        qv[i] = Q8Item{};
+        qv[i] = Q8Piece<16>{};
+        if constexpr (!kScaled) qd[i] = 0;
         if (rr < BN && k < p.k) {
           const unsigned char* b = weight_base(rr) + (size_t)(k / 32) * kBlockBytes;
-          qv[i].d = load_any<uint16_t>(b);
-          const uintx4 q = load_any<uintx4>(b + 2 + k % 32);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) qv[i].q[e] = q[e];
+          qv[i].load(b, k % 32, edge);
+          if constexpr (!kScaled) qd[i] = *reinterpret_cast<const uint16_t*>(b);
         }
       }
     } else if constexpr (!kDmaW) {
 #pragma unroll
       for (int i = 0; i < kWItems; ++i) {
-        const int item = tid + 256 * i, rr = item / kChunks, c = item % kChunks;
+        const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
         wv[i] = load_chunk<T, W>(reinterpret_cast<const W*>(weight_base(rr)), k0 + N * c, p.k);
       }
     }
@@ -192,18 +228,21 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(Linear p) {
     if constexpr (!DMA) {
 #pragma unroll
       for (int i = 0; i < kXItems; ++i) {
-        const int item = tid + 256 * i, rr = item / kChunks, c = item % kChunks;
+        const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
         *reinterpret_cast<uintx4*>(lds.x[buf] + rr * kRowBytes + 16 * (c ^ (rr & 7))) = xv[i];
       }
     }
     if constexpr (kIsQ8<W>) {
 #pragma unroll
       for (int i = 0; i < kWItems; ++i) {
-        const int item = tid + 256 * i, rr = item / (BK / 16), part = item % (BK / 16);
+        const int item = tid + THREADS * i, rr = item / (BK / 16), part = item % (BK / 16);
         if (rr >= BN) continue;
-        const float d = fp16_bits_to_fp32(qv[i].d);
-        if constexpr (kScaled)
-          if (part % 2 == 0) lds.d[buf][part / 2 * BN + rr] = d;
+        float d = 1.0f;
+        if constexpr (kScaled) {
+          if (part % 2 == 0) lds.d[buf][part / 2 * BN + rr] = qv[i].scale();
+        } else {
+          d = fp16_bits_to_fp32(qd[i]);
+        }
 #pragma unroll
         for (int c = 0; c < 16 / N; ++c) {
           union {
@@ -212,8 +251,7 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(Linear p) {
           } o;
 #pragma unroll
           for (int e = 0; e < N; ++e) {
-            const int at = N * c + e;
-            const float q = (float)(int8_t)(qv[i].q[at / 4] >> (8 * (at % 4)));
+            const float q = qv[i].value(N * c + e);
             o.v[e] = (T)(kScaled ? q : d * q);
           }
           *reinterpret_cast<uintx4*>(lds.w[buf] + rr * kRowBytes +
@@ -223,60 +261,70 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(Linear p) {
     } else if constexpr (!kDmaW) {
 #pragma unroll
       for (int i = 0; i < kWItems; ++i) {
-        const int item = tid + 256 * i, rr = item / kChunks, c = item % kChunks;
+        const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
         *reinterpret_cast<uintx4*>(lds.w[buf] + rr * kRowBytes + 16 * (c ^ weight_key<JBG>(rr))) = wv[i];
       }
     }
   };
   // The same straight to LDS: a wave's load fills 1 KB, 8 rows, lane l the chunk
-  // l % 8 of row l / 8; the swizzle is in which chunk it reads. Chunks past k are zeroed.
-  constexpr int kXDma = DMA ? BM / 32 : 0, kWDma = kDmaW ? BN / 32 : 0;  // per wave
+  // l % 8 of row l / 8; the swizzle is in which chunk it reads. In the last slice
+  // chunks that pass k go through registers, zeros from k on.
+  constexpr int kXDma = DMA ? BM / 8 / WAVES : 0, kWDma = kDmaW ? BN / 8 / WAVES : 0;  // per wave
   uint32_t xoff[DMA ? kXDma : 1], woff[kDmaW ? kWDma : 1];
-  int xc = 0, wc[kDmaW ? kWDma : 1];
-  const unsigned char* wbase[kDmaW ? kWDma : 1];
-  const T* xbase = xrows + row0 * p.ldx;
+  const unsigned char *xbase = nullptr, *wbase[G] = {};
   if constexpr (DMA) {
-    xc = (lane & 7) ^ (lane >> 3);
+    xbase = reinterpret_cast<const unsigned char*>(xrows + row0 * p.ldx);
 #pragma unroll
     for (int i = 0; i < kXDma; ++i) {
       const unsigned rr = 8 * (kXDma * wave + i) + (lane >> 3);
-      xoff[i] = (uint32_t)((min(row0 + rr, p.n - 1) - row0) * p.ldx * sizeof(T)) + 16 * xc;
+      xoff[i] = (uint32_t)((min(row0 + rr, p.n - 1) - row0) * p.ldx * sizeof(T)) + 16 * ((lane & 7) ^ (lane >> 3));
     }
   }
   if constexpr (kDmaW) {
 #pragma unroll
+    for (int z = 0; z < G; ++z) wbase[z] = weight_base(z * COLS);
+#pragma unroll
     for (int i = 0; i < kWDma; ++i) {
-      const int first = 8 * (kWDma * wave + i), rr = first + (lane >> 3);
-      wc[i] = (lane & 7) ^ weight_key<JBG>(rr);
-      wbase[i] = weight_base(first);  // uniform
-      woff[i] = (uint32_t)(weight_base(rr) - wbase[i]) + 16 * wc[i];
+      const int rr = 8 * (kWDma * wave + i) + (lane >> 3);
+      woff[i] = (uint32_t)(weight_base(rr) - weight_base(GATED && rr >= COLS ? COLS : 0)) + 16 * ((lane & 7) ^ weight_key<JBG>(rr));
     }
   }
-  auto lds_at = [](const void* q) {
-    return __builtin_amdgcn_readfirstlane(
-        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)static_cast<const unsigned char*>(q));
+  auto lds_address = [](const void* q) {
+    return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)static_cast<const unsigned char*>(q);
   };
+  const uint32_t lds_x = lds_address(lds.x[0]), lds_w = lds_address(lds.w[0]);
   auto dma = [&](int buf, unsigned k0) {
-    const bool full = k0 + BK <= p.k;
-    const uintx4 zero = {};
+    const uint32_t to_x = lds_x + buf * BM * kRowBytes + 1024 * kXDma * wave, to_w = lds_w + buf * BN * kRowBytes + 1024 * kWDma * wave;
+    if (k0 + BK <= p.k) {  // uniform; straight-line code
+      if constexpr (DMA) {
+#pragma unroll
+        for (int i = 0; i < kXDma; ++i) dma16(xbase + k0 * sizeof(T), xoff[i], to_x + 1024 * i);
+      }
+      if constexpr (kDmaW) {
+#pragma unroll
+        for (int i = 0; i < kWDma; ++i)
+          dma16(wbase[GATED && 8 * (kWDma * wave + i) >= COLS] + k0 * sizeof(T), woff[i], to_w + 1024 * i);
+      }
+      return;
+    }
+    auto piece = [&](const unsigned char* base, uint32_t off, unsigned chunk, uint32_t to, unsigned char* place) {
+      if (k0 + N * chunk + N <= p.k)
+        dma16(base + k0 * sizeof(T), off, to);
+      else
+        *reinterpret_cast<uintx4*>(place + 16 * lane) =
+            load_chunk<T, T>(reinterpret_cast<const T*>(base + off - 16 * chunk), k0 + N * chunk, p.k);
+    };
     if constexpr (DMA) {
 #pragma unroll
-      for (int i = 0; i < kXDma; ++i) {
-        unsigned char* to = lds.x[buf] + 1024 * (kXDma * wave + i);
-        if (full || k0 + N * xc < p.k)
-          dma16(xbase + k0, xoff[i], lds_at(to));
-        else
-          *reinterpret_cast<uintx4*>(to + 16 * lane) = zero;
-      }
+      for (int i = 0; i < kXDma; ++i)
+        piece(xbase, xoff[i], (lane & 7) ^ (lane >> 3), to_x + 1024 * i, lds.x[buf] + 1024 * (kXDma * wave + i));
     }
     if constexpr (kDmaW) {
 #pragma unroll
       for (int i = 0; i < kWDma; ++i) {
-        unsigned char* to = lds.w[buf] + 1024 * (kWDma * wave + i);
-        if (full || k0 + N * wc[i] < p.k)
-          dma16(wbase[i] + k0 * sizeof(T), woff[i], lds_at(to));
-        else
-          *reinterpret_cast<uintx4*>(to + 16 * lane) = zero;
+        const int at = kWDma * wave + i;
+        piece(wbase[GATED && 8 * at >= COLS], woff[i], (lane & 7) ^ weight_key<JBG>(8 * at + (lane >> 3)), to_w + 1024 * i,
+              lds.w[buf] + 1024 * at);
       }
     }
   };
@@ -317,24 +365,33 @@ __global__ void __launch_bounds__(256) linear_tile_kernel(Linear p) {
             acc[i][j] = mfma16<T>(a[j], b[i], acc[i][j]);
           }
         }
+        if constexpr (kScaled) __builtin_amdgcn_sched_barrier(0);  // the dots of a block of columns at a time
       }
     }
   };
 
   const unsigned slices = (p.k + BK - 1) / BK;
-  dma(0, 0);
+#pragma unroll
+  for (int i = 0; i < NBUF - 1; ++i)
+    if (i < (int)slices) dma(i, i * BK);
   load(0);
   put(0);
+  int buf = 0;
   for (unsigned s = 0; s < slices; ++s) {
-    // The slice is in its buffer, and the other buffer has been read.
-    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (s + 1 < slices) {
-      dma((s + 1) & 1, (s + 1) * BK);
-      load((s + 1) * BK);
+    // The slice is in its buffer (those behind it may be on their way: a slice is
+    // kXDma + kWDma loads of a wave, or drained), and the buffer before it has been read.
+    if constexpr (DMA) {
+      if (NBUF > 2 && s + NBUF - 2 < slices)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 2) * (kXDma + kWDma)) : "memory");
+      else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    multiply(s & 1);
+    __syncthreads();
+    if (s + NBUF - 1 < slices) dma(buf == 0 ? NBUF - 1 : buf - 1, (s + NBUF - 1) * BK);
+    if (s + 1 < slices) load((s + 1) * BK);
+    multiply(buf);
     if (s + 1 < slices) put((s + 1) & 1);
+    buf = buf + 1 < NBUF ? buf + 1 : 0;
   }
 #pragma unroll
   for (int i = 0; i < IB; ++i) {
@@ -362,41 +419,36 @@ template <class T, class W>
 struct FewWeights {  // a step of a row: 32 values (fp32: two chunks of 16)
   static constexpr int kChunk = __is_same(T, float) ? 2 : 1;
   uintx4 v[kChunk];
-  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end) {
+  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end, bool) {
 #pragma unroll
     for (int c = 0; c < kChunk; ++c)
       v[c] = load_chunk<T, W>(reinterpret_cast<const W*>(row), k + kPer16<T> * (4 * c + g), end);
   }
-  __device__ __forceinline__ uintx4 get(int c) const { return v[c]; }
+  __device__ __forceinline__ float scale() const { return 1.0f; }
+  __device__ __forceinline__ uintx4 get(int c, float) const { return v[c]; }
 };
 template <class T>
 struct FewWeights<T, Q8> {
-  uint32_t q[2];
-  uint32_t d;
-  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end) {
-    q[0] = q[1] = d = 0;
-    if (k >= end) return;
-    const unsigned char* b = row + (size_t)(k / 32) * kBlockBytes;
-    d = load_any<uint16_t>(b);
-    if constexpr (__is_same(T, float)) {  // values 4 g .. and 16 + 4 g ..
-      q[0] = load_any<uint32_t>(b + 2 + 4 * g);
-      q[1] = load_any<uint32_t>(b + 18 + 4 * g);
-    } else {
-      const uint2 v = load_any<uint2>(b + 2 + 8 * g);
-      q[0] = v.x;
-      q[1] = v.y;
+  static constexpr int N = kPer16<T>;
+  Q8Piece<N> q[__is_same(T, float) ? 2 : 1];
+  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end, bool edge) {
+#pragma unroll
+    for (int c = 0; c < (N == 4 ? 2 : 1); ++c) {
+      q[c] = Q8Piece<N>{};
+      if (k < end) q[c].load(row + (size_t)(k / 32) * kBlockBytes, 16 * c + N * g, edge);
     }
   }
-  __device__ __forceinline__ uintx4 get(int c) const {
-    constexpr int N = kPer16<T>;
+  // The block's scale, which the first lane of its four loaded.
+  __device__ __forceinline__ float scale() const { return __shfl(q[0].scale(), threadIdx.x & 15, 64); }
+  __device__ __forceinline__ uintx4 get(int c, float d) const {
     union {
       uintx4 all;
       T v[N];
     } o;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const float f = (float)(int8_t)(q[N == 4 ? c : e / 4] >> (8 * (e % 4)));
-      o.v[e] = (T)(N == 4 ? fp16_bits_to_fp32(d) * f : f);
+      const float f = q[c].value(e);
+      o.v[e] = (T)(N == 4 ? d * f : f);
     }
     return o.all;
   }
@@ -422,6 +474,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
     else
       wrow[z] += row * p.ldw * sizeof(W);
   }
+  const bool edge = col0 == 0 || col0 + 16 >= p.m;
   const T* xrow[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) xrow[i] = static_cast<const T*>(p.x) + min(row0 + 16 * i + r, p.n - 1) * p.ldx;
@@ -438,7 +491,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
     if (step >= steps) return;  // uniform
     const unsigned k = 32 * step;
 #pragma unroll
-    for (int z = 0; z < G; ++z) w[slot][z].load(wrow[z], k, g, p.k);
+    for (int z = 0; z < G; ++z) w[slot][z].load(wrow[z], k, g, p.k, edge);
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
@@ -452,20 +505,19 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
       if (step + kFewWaves * s >= steps) break;  // uniform
 #pragma unroll
       for (int z = 0; z < G; ++z) {
-        floatx4 d;
-        if constexpr (kScaled) {  // of the lane's four columns 4 g .., from the lanes that loaded them
+        const float d = w[s][z].scale();  // of column r
+        uintx4 a[kChunk];
 #pragma unroll
-          for (int v = 0; v < 4; ++v) d[v] = fp16_bits_to_fp32(__shfl((int)w[s][z].d, 4 * g + v, 64));
-        }
+        for (int c = 0; c < kChunk; ++c) a[c] = w[s][z].get(c, d);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
-          if constexpr (kScaled) {
-            const floatx4 dot = mfma16<T>(w[s][z].get(0), x[s][i][0], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+          if constexpr (kScaled) {  // rows 4 g .. of column r
+            const floatx4 dot = mfma16<T>(x[s][i][0], a[0], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
-            for (int v = 0; v < 4; ++v) acc[z][i][v] = __builtin_fmaf(dot[v], d[v], acc[z][i][v]);
-          } else {
+            for (int v = 0; v < 4; ++v) acc[z][i][v] = __builtin_fmaf(dot[v], d, acc[z][i][v]);
+          } else {  // columns 4 g .. of row r
 #pragma unroll
-            for (int c = 0; c < kChunk; ++c) acc[z][i] = mfma16<T>(w[s][z].get(c), x[s][i][c], acc[z][i]);
+            for (int c = 0; c < kChunk; ++c) acc[z][i] = mfma16<T>(a[c], x[s][i][c], acc[z][i]);
           }
         }
       }
@@ -481,9 +533,18 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
   float sum[2][4];
 #pragma unroll
   for (int z = 0; z < 2; ++z) {
-    floatx4 s = part[0][z < G ? z : 0][wave][lane];
+    floatx4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int u = 1; u < kFewWaves; ++u) s = s + part[u][z < G ? z : 0][wave][lane];
+    for (int u = 0; u < kFewWaves; ++u) {
+      const floatx4* from = part[u][z < G ? z : 0][wave];
+      if constexpr (kScaled) {  // row r of column 4 g + v: lane 16 (r / 4) + column, element r % 4
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          s[v] = s[v] + reinterpret_cast<const float*>(from)[4 * (16 * (r >> 2) + 4 * g + v) + (r & 3)];
+      } else {
+        s = s + from[lane];
+      }
+    }
 #pragma unroll
     for (int v = 0; v < 4; ++v) sum[z][v] = s[v];
   }
@@ -492,8 +553,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
 
 // ------------------------------------------------------------------ launches
 
-inline bool on16(const void* p, uint64_t ld, size_t size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0;
+inline bool on4(const void* p, uint64_t ld, size_t size) {
+  return reinterpret_cast<uintptr_t>(p) % 4 == 0 && ld * size % 4 == 0 && ld < 1u << 21;
 }
 
 template <class T, class W, bool GATED>
@@ -502,7 +563,8 @@ hipError_t launch_linear_form(const Linear& p, hipStream_t st) {
   auto count = [](unsigned n, unsigned by) { return (n + by - 1) / by; };
   // n m <= 2^32: at most 2^24 + 2^21 workgroups of any form.
   constexpr unsigned kSmallCols = GATED ? 32 : 64, kLargeCols = GATED ? 64 : 128;
-  if (p.n <= 64 || count(p.n, 64) * count(p.m, kSmallCols) < kCus / 2) {
+  const char* ff = getenv("EG2_TILE");
+  if (ff ? atoi(ff) == 16 : p.n <= 64 || count(p.n, 64) * count(p.m, kSmallCols) < kCus / 2) {
     const unsigned nb = p.n <= 16 ? 1 : p.n <= 32 ? 2 : 4;
     const unsigned groups = count(p.n, 16 * nb) * count(p.m, 16);
     if (nb == 1)
@@ -513,26 +575,30 @@ hipError_t launch_linear_form(const Linear& p, hipStream_t st) {
       linear_few_kernel<T, W, GATED, 4><<<groups, 64 * kFewWaves, 0, st>>>(p);
     return hipGetLastError();
   }
-  // Straight to LDS where rows lie on 16 bytes, hold whole chunks, and a tile's rows within 2 GiB.
-  bool dma = on16(p.x, p.ldx, sizeof(T)) && p.k % kPer16<T> == 0 && p.ldx < 1u << 20;
-  if constexpr (__is_same(T, W)) {
-    dma = dma && p.ldw < 1u << 20;
-    for (int z = 0; z < (GATED ? 2 : 1); ++z) dma = dma && on16(p.w[z], p.ldw, sizeof(T));
-  }
-  const bool large = count(p.n, 128) * count(p.m, kLargeCols) >= kCus;
-  const unsigned tiles = large ? count(p.n, 128) * count(p.m, kLargeCols) : count(p.n, 64) * count(p.m, kSmallCols);
-  if (large) {
+  // Straight to LDS where rows lie on 4 bytes, and a tile's within 2^31.
+  bool dma = on4(p.x, p.ldx, sizeof(T));
+  if constexpr (__is_same(T, W))
+    for (int z = 0; z < (GATED ? 2 : 1); ++z) dma = dma && on4(p.w[z], p.ldw, sizeof(T));
+  constexpr bool kSame = __is_same(T, W);
+  auto tiles = [&](auto bm, auto bn, auto wm, auto wn, auto nbuf) {
+    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+    constexpr int NBUF = kSame ? decltype(nbuf)::value : 2;
+    const unsigned groups = count(p.n, BM) * count(p.m, BN / (GATED ? 2 : 1));
     if (dma)
-      linear_tile_kernel<T, W, GATED, true, 128, 128><<<tiles, 256, 0, st>>>(p);
+      linear_tile_kernel<T, W, GATED, true, BM, BN, WM, WN, NBUF><<<groups, 64 * WM * WN, 0, st>>>(p);
     else
-      linear_tile_kernel<T, W, GATED, false, 128, 128><<<tiles, 256, 0, st>>>(p);
-  } else {
-    if (dma)
-      linear_tile_kernel<T, W, GATED, true, 64, 64><<<tiles, 256, 0, st>>>(p);
-    else
-      linear_tile_kernel<T, W, GATED, false, 64, 64><<<tiles, 256, 0, st>>>(p);
-  }
-  return hipGetLastError();
+      linear_tile_kernel<T, W, GATED, false, BM, BN, WM, WN, 2><<<groups, 64 * WM * WN, 0, st>>>(p);
+    return hipGetLastError();
+  };
+  const char* f = getenv("EG2_TILE");
+  const int form = f ? atoi(f) : 0;
+  const unsigned of128 = count(p.n, 128) * count(p.m, kLargeCols);
+  if constexpr (kSame && !__is_same(T, float))
+    if (form ? form == 256 : count(p.n, 256) * count(p.m, 2 * kLargeCols) >= kCus)
+      return tiles(Const<256>{}, Const<256>{}, Const<2>{}, Const<4>{}, Const<2>{});
+  if (form ? form == 128 : of128 >= kCus) return tiles(Const<128>{}, Const<128>{}, Const<2>{}, Const<2>{}, Const<2>{});
+  if (form == 1284) return tiles(Const<128>{}, Const<128>{}, Const<2>{}, Const<2>{}, Const<4>{});
+  return tiles(Const<64>{}, Const<64>{}, Const<2>{}, Const<2>{}, Const<4>{});
 }
 
 // Every weight type of activations T (the record's types have been checked).
