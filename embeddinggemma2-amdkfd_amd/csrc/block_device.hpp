@@ -23,17 +23,12 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float over_one_plus_exp(float z, float t) {
   return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * t));
 }
-__device__ __forceinline__ float activate(float z, unsigned act) {
-  switch (act) {
-    case EG2_ACT_GELU:
-      return over_one_plus_exp(z, 2.0f * gelu_inner(z));
-    case EG2_ACT_SILU:
-      return over_one_plus_exp(z, z);
-    case EG2_ACT_RELU:
-      return z < 0.0f ? 0.0f : z;
-    default:
-      return z;
-  }
+template <unsigned ACT>
+__device__ __forceinline__ float activate(float z) {
+  if constexpr (ACT == EG2_ACT_GELU) return over_one_plus_exp(z, 2.0f * gelu_inner(z));
+  if constexpr (ACT == EG2_ACT_SILU) return over_one_plus_exp(z, z);
+  if constexpr (ACT == EG2_ACT_RELU) return z < 0.0f ? 0.0f : z;
+  return z;
 }
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -72,6 +67,21 @@ template <int N>
 struct Const {
   static constexpr int value = N;
 };
+
+// Calls f with the Const of an activation id: one branch around a whole epilogue.
+template <class F>
+__device__ __forceinline__ void with_activation(unsigned act, F f) {
+  switch (act) {
+    case EG2_ACT_GELU:
+      return f(Const<EG2_ACT_GELU>{});
+    case EG2_ACT_SILU:
+      return f(Const<EG2_ACT_SILU>{});
+    case EG2_ACT_RELU:
+      return f(Const<EG2_ACT_RELU>{});
+    default:
+      return f(Const<EG2_ACT_NONE>{});
+  }
+}
 
 // Calls f with a value of the C++ type of an EG2_TYPE_ id of activations.
 template <class F>

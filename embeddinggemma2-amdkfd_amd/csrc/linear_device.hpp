@@ -55,41 +55,58 @@ __device__ __forceinline__ uintx4 load_chunk(const W* row, unsigned k, unsigned 
   return r.all;
 }
 
+// The biases of COLS columns from `col` on (the last one past the end; 0 where there is none).
+template <int COLS>
+struct Biases {
+  float v[COLS];
+  __device__ __forceinline__ Biases(const float* bias, unsigned col, unsigned m) {
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) v[e] = bias ? bias[min(col + e, m - 1)] : 0.0f;
+  }
+};
+
 // The output of a lane: COLS consecutive columns of one row, from their sums.
-template <class T, bool GATED, int COLS>
+template <class T, bool GATED, unsigned ACT, int COLS>
 __device__ __forceinline__ void finish(const Linear& p, unsigned row, unsigned col, const float (&a)[COLS],
-                                       const float (&b)[COLS]) {
-  static_assert(COLS % 4 == 0, "");
+                                       const float (&b)[COLS], const Biases<COLS>& a_bias, const Biases<COLS>& b_bias) {
   if (row >= p.n || col >= p.m) return;
+  constexpr int N = COLS % kPer16<T> == 0 ? kPer16<T> : 4;  // values of a store
+  static_assert(COLS % 4 == 0, "");
+  struct alignas(sizeof(T) * N) Some {
+    T v[N];
+  };
   T* y = static_cast<T*>(p.y) + row * p.ldy + col;
   const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr + col : nullptr;
-  struct alignas(sizeof(T) * 4) Four {
-    T v[4];
-  };
-  auto on = [](const void* q) { return q == nullptr || reinterpret_cast<uintptr_t>(q) % sizeof(Four) == 0; };
+  auto on = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % sizeof(Some) == 0; };
   const bool whole = col + COLS <= p.m && on(y) && on(r);
+  float z[COLS];
 #pragma unroll
-  for (int c = 0; c < COLS; c += 4) {
-    Four res, out;
-    if (r && whole) res = *reinterpret_cast<const Four*>(r + c);
+  for (int e = 0; e < COLS; ++e) {
+    z[e] = activate<ACT>(a[e] + a_bias.v[e]);
+    if constexpr (GATED) z[e] = z[e] * (b[e] + b_bias.v[e]);
+  }
+  if (whole) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const unsigned at = min(col + c + e, p.m - 1);
-      float z = a[c + e];
-      if (p.bias[0]) z = z + p.bias[0][at];
-      z = activate(z, p.act);
-      if constexpr (GATED) {
-        float u = b[c + e];
-        if (p.bias[1]) u = u + p.bias[1][at];
-        z = z * u;
-      } else if (r) {
-        if (!whole) res.v[e] = r[at - col];
-        z = z + to_float(res.v[e]);
-      }
-      out.v[e] = (T)z;
-      if (!whole && col + c + e < p.m) y[c + e] = out.v[e];
+    for (int c = 0; c < COLS; c += N) {
+      if constexpr (!GATED)
+        if (r) {
+          const Some s = *reinterpret_cast<const Some*>(r + c);
+#pragma unroll
+          for (int e = 0; e < N; ++e) z[c + e] = z[c + e] + to_float(s.v[e]);
+        }
+      Some out;
+#pragma unroll
+      for (int e = 0; e < N; ++e) out.v[e] = (T)z[c + e];
+      *reinterpret_cast<Some*>(y + c) = out;
     }
-    if (whole) *reinterpret_cast<Four*>(y + c) = out;
+  } else {
+#pragma unroll
+    for (int e = 0; e < COLS; ++e) {
+      if (col + e >= p.m) break;
+      if constexpr (!GATED)
+        if (r) z[e] = z[e] + to_float(r[e]);
+      y[e] = (T)z[e];
+    }
   }
 }
 
@@ -393,18 +410,22 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(Linear p) {
     if (s + 1 < slices) put((s + 1) & 1);
     buf = buf + 1 < NBUF ? buf + 1 : 0;
   }
+  const unsigned col = col0 + wn * (16 * JBG) + 4 * JBG * g;
+  const Biases<4 * JBG> a_bias(p.bias[0], col, p.m), b_bias(GATED ? p.bias[1] : nullptr, col, p.m);
+  with_activation(p.act, [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < IB; ++i) {
-    float a[4 * JBG], b[4 * JBG];
+    for (int i = 0; i < IB; ++i) {
+      float a[4 * JBG], b[4 * JBG];
 #pragma unroll
-    for (int j = 0; j < JBG; ++j)
+      for (int j = 0; j < JBG; ++j)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        a[4 * j + v] = acc[i][j][v];
-        b[4 * j + v] = acc[i][JB - JBG + j][v];
-      }
-    finish<T, GATED, 4 * JBG>(p, row0 + 16 * (IB * wm + i) + r, col0 + wn * (16 * JBG) + 4 * JBG * g, a, b);
-  }
+        for (int v = 0; v < 4; ++v) {
+          a[4 * j + v] = acc[i][j][v];
+          b[4 * j + v] = acc[i][JB - JBG + j][v];
+        }
+      finish<T, GATED, decltype(act)::value>(p, row0 + 16 * (IB * wm + i) + r, col, a, b, a_bias, b_bias);
+    }
+  });
 }
 
 // ------------------------------------------------------------------ few rows
@@ -548,7 +569,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
 #pragma unroll
     for (int v = 0; v < 4; ++v) sum[z][v] = s[v];
   }
-  finish<T, GATED, 4>(p, row0 + 16 * wave + r, col0 + 4 * g, sum[0], sum[1]);
+  const unsigned col = col0 + 4 * g;
+  const Biases<4> a_bias(p.bias[0], col, p.m), b_bias(GATED ? p.bias[1] : nullptr, col, p.m);
+  with_activation(p.act, [&](auto act) {
+    finish<T, GATED, decltype(act)::value>(p, row0 + 16 * wave + r, col, sum[0], sum[1], a_bias, b_bias);
+  });
 }
 
 // ------------------------------------------------------------------ launches
