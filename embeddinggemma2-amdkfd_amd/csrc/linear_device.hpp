@@ -13,7 +13,6 @@
 
 #include <hip/hip_runtime.h>
 
-#include <cstdlib>
 #include "block_device.hpp"
 #include "eg2_block.hpp"
 
@@ -100,13 +99,17 @@ __device__ __forceinline__ void finish(const Linear& p, unsigned row, unsigned c
       *reinterpret_cast<Some*>(y + c) = out;
     }
   } else {
+    if constexpr (!GATED)
+      if (r) {  // all on their way at once
+        T v[COLS];
 #pragma unroll
-    for (int e = 0; e < COLS; ++e) {
-      if (col + e >= p.m) break;
-      if constexpr (!GATED)
-        if (r) z[e] = z[e] + to_float(r[e]);
-      y[e] = (T)z[e];
-    }
+        for (int e = 0; e < COLS; ++e) v[e] = r[min((unsigned)e, p.m - 1 - col)];
+#pragma unroll
+        for (int e = 0; e < COLS; ++e) z[e] = z[e] + to_float(v[e]);
+      }
+#pragma unroll
+    for (int e = 0; e < COLS; ++e)
+      if (col + e < p.m) y[e] = (T)z[e];
   }
 }
 
@@ -149,7 +152,7 @@ struct Q8Piece {
 //
 // BM rows of x times BN rows of the weights (of a gated pair BN / 2 of each
 // matrix) per workgroup of WM x WN waves, each 16 x 16 blocks over its
-// part. Slices of 128 bytes of every row go through NBUF LDS buffers, all but one
+// part, or of WK times as many, each share over every WK-th slice of k, added at the end. Slices of 128 bytes of every row go through NBUF LDS buffers, all but one
 // on their way while one is multiplied. The 16-byte chunks of a row are
 // swizzled so that the 16 rows of a fragment read lie on distinct banks. Rows on
 // 4 bytes go straight to LDS (DMA), others and what has to be decoded through
@@ -167,10 +170,10 @@ __device__ __forceinline__ int weight_key(int row) {
   return (row & 3) | ((row / (4 * JBG)) & 1) << 2;
 }
 
-template <class T, class W, bool GATED, bool DMA, int BM, int BN, int WM, int WN, int NBUF>
-__global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(Linear p) {
+template <class T, class W, bool GATED, bool DMA, int BM, int BN, int WM, int WN, int WK, int NBUF>
+__global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p) {
   constexpr int G = GATED ? 2 : 1, COLS = BN / G;  // columns of y
-  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;
+  constexpr int WAVES = WM * WN, THREADS = 64 * WAVES;  // of a share of k
   constexpr int IB = BM / 16 / WM, JB = BN / 16 / WN, JBG = JB / G;
   constexpr int N = kPer16<T>, BK = kChunks * N;  // values per chunk and slice
   constexpr bool kScaled = kIsQ8<W> && !__is_same(T, float);
@@ -182,9 +185,15 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(Linear p) {
     alignas(16) unsigned char w[NBUF][BN * kRowBytes];
     alignas(16) float d[kScaled ? 2 : 1][kScaled ? kBlocks * BN : 4];
   };
-  __shared__ Lds lds;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  __shared__ union {
+    Lds share[WK];
+    floatx4 part[WK > 1 ? WK - 1 : 1][WK > 1 ? WAVES * IB * JB : 1][64];
+  } all;
+  const int wk = WK > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / THREADS) : 0;
+  const int tid = WK > 1 ? threadIdx.x % THREADS : threadIdx.x;
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15, wm = wave / WN, wn = wave % WN;
+  Lds& lds = all.share[wk];
 
   // Workgroups go round the 8 XCDs; each XCD takes a run of tiles, eight rows
   // of tiles down before the next column, so that its L2 serves both operands.
@@ -387,28 +396,47 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_tile_kernel(Linear p) {
     }
   };
 
-  const unsigned slices = (p.k + BK - 1) / BK;
+  // A share takes every WK-th slice.
+  const unsigned slices = (p.k + BK - 1) / BK, turns = (slices + WK - 1) / WK;
 #pragma unroll
   for (int i = 0; i < NBUF - 1; ++i)
-    if (i < (int)slices) dma(i, i * BK);
-  load(0);
+    if (wk + i * WK < slices) dma(i, (wk + i * WK) * BK);
+  load(wk * BK);
   put(0);
   int buf = 0;
-  for (unsigned s = 0; s < slices; ++s) {
+  for (unsigned turn = 0; turn < turns; ++turn) {
+    const unsigned s = wk + turn * WK;
     // The slice is in its buffer (those behind it may be on their way: a slice is
     // kXDma + kWDma loads of a wave, or drained), and the buffer before it has been read.
     if constexpr (DMA) {
-      if (NBUF > 2 && s + NBUF - 2 < slices)
+      if (NBUF > 2 && s + (NBUF - 2) * WK < slices)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NBUF - 2) * (kXDma + kWDma)) : "memory");
       else
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
     __syncthreads();
-    if (s + NBUF - 1 < slices) dma(buf == 0 ? NBUF - 1 : buf - 1, (s + NBUF - 1) * BK);
-    if (s + 1 < slices) load((s + 1) * BK);
-    multiply(buf);
-    if (s + 1 < slices) put((s + 1) & 1);
+    if (s + (NBUF - 1) * WK < slices) dma(buf == 0 ? NBUF - 1 : buf - 1, (s + (NBUF - 1) * WK) * BK);
+    if (s + WK < slices) load((s + WK) * BK);
+    if (s < slices) multiply(buf);
+    if (s + WK < slices) put(buf ^ 1);  // of two
     buf = buf + 1 < NBUF ? buf + 1 : 0;
+  }
+  if constexpr (WK > 1) {
+    __syncthreads();
+    if (wk > 0) {
+#pragma unroll
+      for (int i = 0; i < IB; ++i)
+#pragma unroll
+        for (int j = 0; j < JB; ++j) all.part[wk - 1][(wave * IB + i) * JB + j][lane] = acc[i][j];
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int i = 0; i < IB; ++i)
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int w = 1; w < WK; ++w) acc[i][j] = acc[i][j] + all.part[w - 1][(wave * IB + i) * JB + j][lane];
   }
   const unsigned col = col0 + wn * (16 * JBG) + 4 * JBG * g;
   const Biases<4 * JBG> a_bias(p.bias[0], col, p.m), b_bias(GATED ? p.bias[1] : nullptr, col, p.m);
@@ -585,45 +613,43 @@ inline bool on4(const void* p, uint64_t ld, size_t size) {
 template <class T, class W, bool GATED>
 hipError_t launch_linear_form(const Linear& p, hipStream_t st) {
   constexpr unsigned kCus = 256;
+  constexpr bool k32 = __is_same(T, float);
   auto count = [](unsigned n, unsigned by) { return (n + by - 1) / by; };
   // n m <= 2^32: at most 2^24 + 2^21 workgroups of any form.
-  constexpr unsigned kSmallCols = GATED ? 32 : 64, kLargeCols = GATED ? 64 : 128;
-  const char* ff = getenv("EG2_TILE");
-  if (ff ? atoi(ff) == 16 : p.n <= 64 || count(p.n, 64) * count(p.m, kSmallCols) < kCus / 2) {
-    const unsigned nb = p.n <= 16 ? 1 : p.n <= 32 ? 2 : 4;
-    const unsigned groups = count(p.n, 16 * nb) * count(p.m, 16);
-    if (nb == 1)
-      linear_few_kernel<T, W, GATED, 1><<<groups, 64 * kFewWaves, 0, st>>>(p);
-    else if (nb == 2)
-      linear_few_kernel<T, W, GATED, 2><<<groups, 64 * kFewWaves, 0, st>>>(p);
-    else
-      linear_few_kernel<T, W, GATED, 4><<<groups, 64 * kFewWaves, 0, st>>>(p);
+  auto few = [&](auto blocks) {
+    constexpr int NB = decltype(blocks)::value;
+    linear_few_kernel<T, W, GATED, NB><<<count(p.n, 16 * NB) * count(p.m, 16), 64 * kFewWaves, 0, st>>>(p);
     return hipGetLastError();
-  }
+  };
+  const uint64_t down16 = count(p.n, 16), across16 = count(p.m, 16);
+  if (p.n <= 16 || down16 * across16 <= 2 * kCus) return few(Const<1>{});
+  if (p.n <= 32 || (k32 && (down16 + 1) / 2 * across16 <= 2 * kCus)) return few(Const<2>{});
+  if (k32 && (down16 + 3) / 4 * across16 <= 2 * kCus) return few(Const<4>{});
+  constexpr unsigned kSmallCols = GATED ? 32 : 64, kLargeCols = GATED ? 64 : 128;
   // Straight to LDS where rows lie on 4 bytes, and a tile's within 2^31.
   bool dma = on4(p.x, p.ldx, sizeof(T));
   if constexpr (__is_same(T, W))
     for (int z = 0; z < (GATED ? 2 : 1); ++z) dma = dma && on4(p.w[z], p.ldw, sizeof(T));
   constexpr bool kSame = __is_same(T, W);
-  auto tiles = [&](auto bm, auto bn, auto wm, auto wn, auto nbuf) {
-    constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+  auto tiles = [&](auto size, auto wm, auto wn, auto wk, auto nbuf) {
+    constexpr int B = decltype(size)::value, WM = decltype(wm)::value, WN = decltype(wn)::value, WK = decltype(wk)::value;
     constexpr int NBUF = kSame ? decltype(nbuf)::value : 2;
-    const unsigned groups = count(p.n, BM) * count(p.m, BN / (GATED ? 2 : 1));
+    const unsigned groups = count(p.n, B) * count(p.m, B / (GATED ? 2 : 1));
     if (dma)
-      linear_tile_kernel<T, W, GATED, true, BM, BN, WM, WN, NBUF><<<groups, 64 * WM * WN, 0, st>>>(p);
+      linear_tile_kernel<T, W, GATED, true, B, B, WM, WN, WK, NBUF><<<groups, 64 * WM * WN * WK, 0, st>>>(p);
     else
-      linear_tile_kernel<T, W, GATED, false, BM, BN, WM, WN, 2><<<groups, 64 * WM * WN, 0, st>>>(p);
+      linear_tile_kernel<T, W, GATED, false, B, B, WM, WN, WK, 2><<<groups, 64 * WM * WN * WK, 0, st>>>(p);
     return hipGetLastError();
   };
-  const char* f = getenv("EG2_TILE");
-  const int form = f ? atoi(f) : 0;
-  const unsigned of128 = count(p.n, 128) * count(p.m, kLargeCols);
-  if constexpr (kSame && !__is_same(T, float))
-    if (form ? form == 256 : count(p.n, 256) * count(p.m, 2 * kLargeCols) >= kCus)
-      return tiles(Const<256>{}, Const<256>{}, Const<2>{}, Const<4>{}, Const<2>{});
-  if (form ? form == 128 : of128 >= kCus) return tiles(Const<128>{}, Const<128>{}, Const<2>{}, Const<2>{}, Const<2>{});
-  if (form == 1284) return tiles(Const<128>{}, Const<128>{}, Const<2>{}, Const<2>{}, Const<4>{});
-  return tiles(Const<64>{}, Const<64>{}, Const<2>{}, Const<2>{}, Const<4>{});
+  if constexpr (kSame && !k32)
+    if (count(p.n, 256) * count(p.m, 2 * kLargeCols) >= kCus)
+      return tiles(Const<256>{}, Const<2>{}, Const<4>{}, Const<1>{}, Const<2>{});
+  if constexpr (!kIsQ8<W> || k32)
+    if (count(p.n, 128) * count(p.m, kLargeCols) >= kCus)
+      return tiles(Const<128>{}, Const<2>{}, Const<2>{}, Const<1>{}, Const<2>{});
+  if (count(p.n, 64) * count(p.m, kSmallCols) < kCus)
+    return tiles(Const<64>{}, Const<2>{}, Const<2>{}, Const<4>{}, Const<2>{});
+  return tiles(Const<64>{}, Const<2>{}, Const<2>{}, Const<k32 ? 2 : 1>{}, Const<k32 ? 2 : 4>{});
 }
 
 // Every weight type of activations T (the record's types have been checked).
