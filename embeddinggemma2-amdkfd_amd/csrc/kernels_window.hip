@@ -12,9 +12,12 @@
 // in that order. Keys and values come straight to LDS, a tile ahead; the 16-bit
 // values are transposed on their way out of it (ds_read_b64_tr_b16).
 //
-// The softmax weights of 16-bit attention are rounded to the type, at most half
-// a step each, as the matrix unit takes them; their sum is formed from the
-// 32-bit ones. The running maximum moves only when a score exceeds it by 2^8
+// The matrix unit takes the softmax weights of 16-bit attention in that type. Where
+// a tile has up to 64 rows they go as the sum of two (PARTS: the weight rounded, and what that
+// left, rounded), which costs nothing that shows there; with 128 rows, bound by the
+// products, as one, rounded by at most half a step, which over many keys adds as much error
+// to a result as its own rounding (rms 2.2e-3 of bf16 against 1.7e-3). The sum is
+// formed from the 32-bit weights. The running maximum moves only when a score exceeds it by 2^8
 // (weights up to 2^8 lose nothing in any type), which spares most of the
 // rescaling of the sums.
 //
@@ -98,7 +101,7 @@ __device__ __forceinline__ uint32_t non_finite_bits(uintx4 v) {
 // DP: head size padded to a multiple of 64. WM x WK waves: WM row groups, each
 // with every key of its share, and WK shares of the keys, joined at the end. BN
 // keys to a tile, NBUF tiles in LDS, all but one on their way.
-template <class T, int DP, int QB, int WM, int WK, int BN, int NBUF>
+template <class T, int DP, int QB, int WM, int WK, int BN, int NBUF, int PARTS>
 __global__ void __launch_bounds__(64 * WM * WK, WM > 1 && DP * (int)sizeof(T) <= 512 ? 2 : 1)
 window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out, float2* part_ml, float c) {
   constexpr bool k32 = __is_same(T, float);
@@ -386,13 +389,17 @@ window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out
       union {
         uintx4 all;
         T v[8];
-      } w[QB][KB / 2];
+      } w[PARTS][QB][KB / 2];
 #pragma unroll
       for (int i = 0; i < QB; ++i)
 #pragma unroll
         for (int kp = 0; kp < KB / 2; ++kp)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[i][kp].v[e] = (T)sc[i][2 * kp + e / 4][e % 4];
+          for (int e = 0; e < 8; ++e) {
+            const float f = sc[i][2 * kp + e / 4][e % 4];
+            w[0][i][kp].v[e] = (T)f;
+            if constexpr (PARTS == 2) w[1][i][kp].v[e] = (T)(f - to_float(w[0][i][kp].v[e]));
+          }
       constexpr int kSteps = KB / 2 * OB / 4;  // of four blocks of dimensions
       uintx4 f[2][4];
       auto load_values = [&](int n) {
@@ -408,7 +415,8 @@ window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out
 #pragma unroll
           for (int i = 0; i < QB; ++i) {
             floatx4& sum = acc[i][n % (OB / 4) * 4 + o];
-            sum = mfma16<T>(f[n & 1][o], w[i][n / (OB / 4)].all, sum);
+#pragma unroll
+            for (int part = PARTS - 1; part >= 0; --part) sum = mfma16<T>(f[n & 1][o], w[part][i][n / (OB / 4)].all, sum);
           }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -419,14 +427,19 @@ window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out
   int buf = 0;
   for (int n = 0; n < turns; ++n) {
     const int t = t0 + wk + n * WK;
+    if constexpr (NBUF == 1) {  // each wave on its own
+      static_assert(NBUF > 1 || WM == 1, "one buffer is not shared");
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (t < t1) stage(0, t);
+    }
     // This tile is in LDS (those behind it may be on their way), and the buffer before it has been read.
-    if (t + (NBUF - 2) * WK < t1)
-      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * 2 * kLoads) : "memory");
+    if (NBUF > 2 && t + (NBUF - 2) * WK < t1)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF > 2 ? NBUF - 2 : 0) * 2 * kLoads) : "memory");
     else
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     if constexpr (WM > 1) __syncthreads();
     const int ahead = t + (NBUF - 1) * WK;
-    if (ahead < t1) stage(buf == 0 ? NBUF - 1 : buf - 1, ahead);
+    if (NBUF > 1 && ahead < t1) stage(buf == 0 ? NBUF - 1 : buf - 1, ahead);
     if (t < t1) {
       const int from = tile_start(t), end = tile_end(t);
       if (active && from < wave_bottom.hi && (end > wave_top.lo || (unsigned)from < p.sinks))
@@ -633,7 +646,8 @@ hipError_t go(const Args& a, hipStream_t st) {
   const unsigned group = a.heads / a.kv_heads, n = (unsigned)((uint64_t)a.rows * group / pl.rows) + a.batch;
   auto whole = [&](auto qb, auto wm, auto wk, auto bn) {
     constexpr int QB = decltype(qb)::value, WM = decltype(wm)::value, WK = decltype(wk)::value, BN = decltype(bn)::value;
-    window_attention_kernel<T, DP, QB, WM, WK, BN, 2><<<n * a.kv_heads, 64 * WM * WK, 0, st>>>(a, n, 1, nullptr, nullptr, c);
+    constexpr int PARTS = k32 || 16 * QB * WM > 64 ? 1 : 2;
+    window_attention_kernel<T, DP, QB, WM, WK, BN, 2, PARTS><<<n * a.kv_heads, 64 * WM * WK, 0, st>>>(a, n, 1, nullptr, nullptr, c);
     return hipGetLastError();
   };
   switch (pl.rows) {
@@ -647,10 +661,10 @@ hipError_t go(const Args& a, hipStream_t st) {
     default:
       break;
   }
-  constexpr int BN = k32 ? 16 : 32, WK = BN * RB <= 8192 ? 4 : 2;  // at most 128 KB of LDS
+  constexpr int BN = k32 ? 16 : 32, WK = 4, NBUF = BN * RB <= 8192 ? 2 : 1;  // at most 128 KB of LDS
   float* sums = static_cast<float*>(a.workspace);
   float2* ml = reinterpret_cast<float2*>(sums + (uint64_t)pl.splits * a.rows * a.heads * a.d);
-  window_attention_kernel<T, DP, 1, 1, WK, BN, 2><<<n * a.kv_heads * pl.splits, 64 * WK, 0, st>>>(a, n, pl.splits, sums, ml, c);
+  window_attention_kernel<T, DP, 1, 1, WK, BN, NBUF, k32 ? 1 : 2><<<n * a.kv_heads * pl.splits, 64 * WK, 0, st>>>(a, n, pl.splits, sums, ml, c);
   if (pl.splits > 1)
     window_join_kernel<T, DP><<<a.rows * a.heads, 256, 0, st>>>(a, pl.splits, sums, ml);
   return hipGetLastError();
