@@ -21,6 +21,14 @@ namespace block {
 
 template <class W>
 constexpr bool kIsQ8 = __is_same(W, Q8);
+template <class T, class W>
+struct OtherThanQ8 {
+  typedef W type;
+};
+template <class T>
+struct OtherThanQ8<T, Q8> {
+  typedef T type;
+};
 
 // Loads at any alignment of the values (one instruction: global loads need none).
 template <class V>
@@ -30,29 +38,38 @@ __device__ __forceinline__ V load_any(const void* p) {
   return v;
 }
 
-// 16 bytes of T from the W values [k, k + kPer16) of a row, zeros from `end` on.
+// The W values [k, k + kPer16<T>) of a row as they lie, zeros from `end` on, and as 16
+// bytes of T. (Converted where they are used, not where they are loaded, which would wait for them.)
 template <class T, class W>
-__device__ __forceinline__ uintx4 load_chunk(const W* row, unsigned k, unsigned end) {
-  constexpr int N = kPer16<T>;
-  union {
-    uintx4 all;
-    T v[N];
-  } r;
-  if (k + N <= end) {
-    if constexpr (__is_same(T, W)) return load_any<uintx4>(row + k);
-    struct Raw {
-      W v[N];
-    };
-    const Raw w = load_any<Raw>(row + k);
+struct Chunk {
+  static constexpr int N = kPer16<T>;
+  struct Raw {
+    W v[N];
+  };
+  Raw raw;
+  __device__ __forceinline__ void load(const W* row, unsigned k) { raw = load_any<Raw>(row + k); }
+  __device__ __forceinline__ void load(const W* row, unsigned k, unsigned end) {
+    if (k + N <= end) {
+      load(row, k);
+    } else {
 #pragma unroll
-    for (int e = 0; e < N; ++e) r.v[e] = (T)to_float(w.v[e]);
-  } else {
-    // The value itself or, past the end, the last one, not used: no branch per value.
-#pragma unroll
-    for (int e = 0; e < N; ++e) r.v[e] = k + e < end ? (T)to_float(row[min(k + e, end - 1)]) : (T)0.0f;
+      for (int e = 0; e < N; ++e) raw.v[e] = k + e < end ? row[min(k + e, end - 1)] : (W)0.0f;
+    }
   }
-  return r.all;
-}
+  __device__ __forceinline__ uintx4 get() const {
+    if constexpr (__is_same(T, W)) {
+      return __builtin_bit_cast(uintx4, raw);
+    } else {
+      union {
+        uintx4 all;
+        T v[N];
+      } r;
+#pragma unroll
+      for (int e = 0; e < N; ++e) r.v[e] = (T)to_float(raw.v[e]);
+      return r.all;
+    }
+  }
+};
 
 // The biases of COLS columns from `col` on (the last one past the end; 0 where there is none).
 template <int COLS>
@@ -217,7 +234,9 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
   // A slice on its way through registers.
   constexpr int kXItems = BM * kChunks / THREADS;
   constexpr int kWItems = kIsQ8<W> ? (BN * BK / 16 + THREADS - 1) / THREADS : BN * kChunks / THREADS;
-  uintx4 xv[DMA ? 1 : kXItems], wv[kIsQ8<W> || kDmaW ? 1 : kWItems];
+  typedef Chunk<T, typename OtherThanQ8<T, W>::type> WChunk;
+  Chunk<T, T> xv[DMA ? 1 : kXItems];
+  WChunk wv[kIsQ8<W> || kDmaW ? 1 : kWItems];
   Q8Piece<16> qv[kIsQ8<W> ? kWItems : 1];
   uint32_t qd[kIsQ8<W> && !kScaled ? kWItems : 1];
   const bool edge = col0 == 0 || col0 + COLS >= p.m;
@@ -226,7 +245,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 #pragma unroll
       for (int i = 0; i < kXItems; ++i) {
         const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
-        xv[i] = load_chunk<T, T>(xrows + min(row0 + rr, p.n - 1) * p.ldx, k0 + N * c, p.k);
+        xv[i].load(xrows + min(row0 + rr, p.n - 1) * p.ldx, k0 + N * c, p.k);
       }
     }
     if constexpr (kIsQ8<W>) {
@@ -246,7 +265,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 #pragma unroll
       for (int i = 0; i < kWItems; ++i) {
         const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
-        wv[i] = load_chunk<T, W>(reinterpret_cast<const W*>(weight_base(rr)), k0 + N * c, p.k);
+        wv[i].load(reinterpret_cast<const W*>(weight_base(rr)), k0 + N * c, p.k);
       }
     }
   };
@@ -255,7 +274,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 #pragma unroll
       for (int i = 0; i < kXItems; ++i) {
         const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
-        *reinterpret_cast<uintx4*>(lds.x[buf] + rr * kRowBytes + 16 * (c ^ (rr & 7))) = xv[i];
+        *reinterpret_cast<uintx4*>(lds.x[buf] + rr * kRowBytes + 16 * (c ^ (rr & 7))) = xv[i].get();
       }
     }
     if constexpr (kIsQ8<W>) {
@@ -288,7 +307,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 #pragma unroll
       for (int i = 0; i < kWItems; ++i) {
         const int item = tid + THREADS * i, rr = item / kChunks, c = item % kChunks;
-        *reinterpret_cast<uintx4*>(lds.w[buf] + rr * kRowBytes + 16 * (c ^ weight_key<JBG>(rr))) = wv[i];
+        *reinterpret_cast<uintx4*>(lds.w[buf] + rr * kRowBytes + 16 * (c ^ weight_key<JBG>(rr))) = wv[i].get();
       }
     }
   };
@@ -336,9 +355,11 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
     auto piece = [&](const unsigned char* base, uint32_t off, unsigned chunk, uint32_t to, unsigned char* place) {
       if (k0 + N * chunk + N <= p.k)
         dma16(base + k0 * sizeof(T), off, to);
-      else
-        *reinterpret_cast<uintx4*>(place + 16 * lane) =
-            load_chunk<T, T>(reinterpret_cast<const T*>(base + off - 16 * chunk), k0 + N * chunk, p.k);
+      else {
+        Chunk<T, T> c;
+        c.load(reinterpret_cast<const T*>(base + off - 16 * chunk), k0 + N * chunk, p.k);
+        *reinterpret_cast<uintx4*>(place + 16 * lane) = c.get();
+      }
     };
     if constexpr (DMA) {
 #pragma unroll
@@ -464,29 +485,30 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 // the order of the operand, and every workgroup's chain is an eighth of k.
 constexpr int kFewWaves = 8;
 
-template <class T, class W>
+template <class T, class W, bool EDGE>
 struct FewWeights {  // a step of a row: 32 values (fp32: two chunks of 16)
   static constexpr int kChunk = __is_same(T, float) ? 2 : 1;
-  uintx4 v[kChunk];
-  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end, bool) {
+  Chunk<T, W> v[kChunk];
+  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g) {
 #pragma unroll
-    for (int c = 0; c < kChunk; ++c)
-      v[c] = load_chunk<T, W>(reinterpret_cast<const W*>(row), k + kPer16<T> * (4 * c + g), end);
+    for (int c = 0; c < kChunk; ++c) v[c].load(reinterpret_cast<const W*>(row), k + kPer16<T> * (4 * c + g));
+  }
+  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end) {
+#pragma unroll
+    for (int c = 0; c < kChunk; ++c) v[c].load(reinterpret_cast<const W*>(row), k + kPer16<T> * (4 * c + g), end);
   }
   __device__ __forceinline__ float scale() const { return 1.0f; }
-  __device__ __forceinline__ uintx4 get(int c, float) const { return v[c]; }
+  __device__ __forceinline__ uintx4 get(int c, float) const { return v[c].get(); }
 };
-template <class T>
-struct FewWeights<T, Q8> {
+template <class T, bool EDGE>
+struct FewWeights<T, Q8, EDGE> {
   static constexpr int N = kPer16<T>;
-  Q8Piece<N> q[__is_same(T, float) ? 2 : 1];
-  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g, unsigned end, bool edge) {
+  Q8Piece<N> q[N == 4 ? 2 : 1];
+  __device__ __forceinline__ void load(const unsigned char* row, unsigned k, unsigned g) {
 #pragma unroll
-    for (int c = 0; c < (N == 4 ? 2 : 1); ++c) {
-      q[c] = Q8Piece<N>{};
-      if (k < end) q[c].load(row + (size_t)(k / 32) * kBlockBytes, 16 * c + N * g, edge);
-    }
+    for (int c = 0; c < (N == 4 ? 2 : 1); ++c) q[c].load(row + (size_t)(k / 32) * kBlockBytes, 16 * c + N * g, EDGE);
   }
+  __device__ __forceinline__ void load(const unsigned char*, unsigned, unsigned, unsigned) {}  // k is a multiple of 32
   // The block's scale, which the first lane of its four loaded.
   __device__ __forceinline__ float scale() const { return __shfl(q[0].scale(), threadIdx.x & 15, 64); }
   __device__ __forceinline__ uintx4 get(int c, float d) const {
@@ -507,7 +529,9 @@ template <class T, class W, bool GATED, int NB>
 __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
   constexpr int G = GATED ? 2 : 1, kChunk = __is_same(T, float) ? 2 : 1;
   constexpr bool kScaled = kIsQ8<W> && !__is_same(T, float);
-  constexpr int kDepth = NB * G >= 4 ? 2 : 4;  // steps on their way
+  // Steps on their way: of a pair two, so that its registers leave room for as many
+  // waves as one matrix has with four (4 x 2048 x 8192 Q8_0: 16.7 us, 18.9 with four).
+  constexpr int kDepth = NB * G >= 4 || GATED ? 2 : 4;
   __shared__ floatx4 part[kFewWaves][G][NB][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
@@ -523,7 +547,6 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
     else
       wrow[z] += row * p.ldw * sizeof(W);
   }
-  const bool edge = col0 == 0 || col0 + 16 >= p.m;
   const T* xrow[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) xrow[i] = static_cast<const T*>(p.x) + min(row0 + 16 * i + r, p.n - 1) * p.ldx;
@@ -533,46 +556,79 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
   for (int z = 0; z < G; ++z)
 #pragma unroll
     for (int i = 0; i < NB; ++i) acc[z][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  const unsigned steps = (p.k + 31) / 32;
-  FewWeights<T, W> w[kDepth][G];
-  uintx4 x[kDepth][NB][kChunk];
-  auto load = [&](int slot, unsigned step) {
-    if (step >= steps) return;  // uniform
-    const unsigned k = 32 * step;
-#pragma unroll
-    for (int z = 0; z < G; ++z) w[slot][z].load(wrow[z], k, g, p.k, edge);
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-      for (int c = 0; c < kChunk; ++c) x[slot][i][c] = load_chunk<T, T>(xrow[i], k + kPer16<T> * (4 * c + g), p.k);
-  };
-#pragma unroll
-  for (int s = 0; s < kDepth; ++s) load(s, wave + kFewWaves * s);
-  for (unsigned step = wave; step < steps; step += kFewWaves * kDepth) {
-#pragma unroll
-    for (int s = 0; s < kDepth; ++s) {
-      if (step + kFewWaves * s >= steps) break;  // uniform
+  auto run = [&](auto edge) {
+    constexpr bool EDGE = decltype(edge)::value != 0;
+    FewWeights<T, W, EDGE> w[kDepth][G];
+    Chunk<T, T> x[kDepth][NB][kChunk];
+    auto multiply = [&](int slot) {
 #pragma unroll
       for (int z = 0; z < G; ++z) {
-        const float d = w[s][z].scale();  // of column r
+        const float d = w[slot][z].scale();  // of column r
         uintx4 a[kChunk];
 #pragma unroll
-        for (int c = 0; c < kChunk; ++c) a[c] = w[s][z].get(c, d);
+        for (int c = 0; c < kChunk; ++c) a[c] = w[slot][z].get(c, d);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           if constexpr (kScaled) {  // rows 4 g .. of column r
-            const floatx4 dot = mfma16<T>(x[s][i][0], a[0], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+            const floatx4 dot = mfma16<T>(x[slot][i][0].get(), a[0], floatx4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
             for (int v = 0; v < 4; ++v) acc[z][i][v] = __builtin_fmaf(dot[v], d, acc[z][i][v]);
           } else {  // columns 4 g .. of row r
 #pragma unroll
-            for (int c = 0; c < kChunk; ++c) acc[z][i] = mfma16<T>(a[c], x[s][i][c], acc[z][i]);
+            for (int c = 0; c < kChunk; ++c) acc[z][i] = mfma16<T>(a[c], x[slot][i][c].get(), acc[z][i]);
           }
         }
       }
-      load(s, step + kFewWaves * (s + kDepth));
+    };
+    // The wave's whole steps: wave, wave + 8, .. The loop's loads stand in no
+    // branch (past the last step it is loaded again), so that a step waits for its own alone.
+    const unsigned steps = p.k / 32, mine = steps > (unsigned)wave ? (steps - wave + kFewWaves - 1) / kFewWaves : 0;
+    auto load = [&](int slot, unsigned n) {
+      const unsigned k = 32 * (wave + kFewWaves * min(n, mine - 1));
+#pragma unroll
+      for (int z = 0; z < G; ++z) w[slot][z].load(wrow[z], k, g);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int c = 0; c < kChunk; ++c) x[slot][i][c].load(xrow[i], k + kPer16<T> * (4 * c + g));
+    };
+    if (mine > kDepth) {
+#pragma unroll
+      for (int s = 0; s < kDepth; ++s) load(s, s);
+      unsigned n = 0;
+      for (; n + kDepth < mine; n += kDepth) {
+#pragma unroll
+        for (int s = 0; s < kDepth; ++s) {
+          multiply(s);
+          load(s, n + kDepth + s);
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < kDepth; ++s)
+        if (n + s < mine) multiply(s);
+    } else {
+#pragma unroll
+      for (int s = 0; s < kDepth; ++s)
+        if (s < (int)mine) load(s, s);
+#pragma unroll
+      for (int s = 0; s < kDepth; ++s)
+        if (s < (int)mine) multiply(s);
     }
-  }
+    // The values past the last whole step.
+    if (p.k % 32 != 0 && steps % kFewWaves == (unsigned)wave) {
+#pragma unroll
+      for (int z = 0; z < G; ++z) w[0][z].load(wrow[z], 32 * steps, g, p.k);
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int c = 0; c < kChunk; ++c) x[0][i][c].load(xrow[i], 32 * steps + kPer16<T> * (4 * c + g), p.k);
+      multiply(0);
+    }
+  };
+  if (kIsQ8<W> && (col0 == 0 || col0 + 16 >= p.m))
+    run(Const<1>{});
+  else
+    run(Const<0>{});
 #pragma unroll
   for (int z = 0; z < G; ++z)
 #pragma unroll
