@@ -68,14 +68,14 @@ bool valid(const eg2_heads_norm_rope_args& a) {
 
 // What the workspace follows from.
 bool valid_sizes(const eg2_window_attention_args& a) {
-  return is_activation_type(a.type) && a.batch > 0 && a.batch <= 65535 && a.rows > 0 && a.rows < 1u << 31 &&
-         a.key_rows > 0 && a.key_rows < 1u << 31 && a.kv_heads > 0 && a.heads > 0 && a.heads <= 4096 &&
+  return is_activation_type(a.type) && a.batch > 0 && a.batch <= 65535 && a.rows > 0 && a.rows <= 1u << 27 &&
+         a.key_rows > 0 && a.key_rows <= 1u << 30 && a.kv_heads > 0 && a.heads > 0 && a.heads <= 4096 &&
          a.heads % a.kv_heads == 0 && a.d >= 8 && a.d <= 256 && a.d % 8 == 0 &&
          (uint64_t)a.rows * a.heads <= (uint64_t)1 << 27 && (uint64_t)a.batch * a.kv_heads <= (uint64_t)1 << 22;
 }
 bool valid(const eg2_window_attention_args& a) {
   if (!valid_sizes(a) || !a.q_offsets || !a.k_offsets || !on(a.q_offsets, 4) || !on(a.k_offsets, 4) ||
-      !on(a.k_lengths, 4) || !std::isfinite(a.scale))
+      !on(a.k_lengths, 4) || !(std::fabs(a.scale) <= 0x1p127f))
     return false;
   const unsigned per16 = 16 / size_of(a.type);
   auto rows_fit = [&](const void* p, uint64_t row, uint64_t head) {

@@ -628,6 +628,9 @@ Plan plan(const Args& a) {
   uint64_t splits = (row <= 128 ? 2 * kCus : kCus) / groups(kFewRows);
   if (splits > span / 64) splits = span / 64;
   if (splits > kMostSplits) splits = kMostSplits;
+  // Sequences without queries have workgroups as well, which end at once: at most 2^22 more of them.
+  const uint64_t most = (1u << 22) / ((uint64_t)a.batch * a.kv_heads);
+  if (splits > most) splits = most;
   if (span < 512) splits = 1;
   return Plan{kFewRows, splits ? (unsigned)splits : 1u};
 }
@@ -642,7 +645,7 @@ hipError_t go(const Args& a, hipStream_t st) {
   constexpr bool k32 = __is_same(T, float);
   constexpr int RB = DP * (int)sizeof(T);
   const float scale = (a.scale < 0.0f ? -a.scale : a.scale) * kLog2e;
-  const float c = scale > 0x1p-100f ? scale : 0x1p-100f;  // 0: equal weights
+  const float c = scale > 0.0f ? scale : 0x1p-149f;  // 0: every finite score below 2^-21, and a hidden key still at -inf
   const unsigned group = a.heads / a.kv_heads, n = (unsigned)((uint64_t)a.rows * group / pl.rows) + a.batch;
   auto whole = [&](auto qb, auto wm, auto wk, auto bn) {
     constexpr int QB = decltype(qb)::value, WM = decltype(wm)::value, WK = decltype(wk)::value, BN = decltype(bn)::value;

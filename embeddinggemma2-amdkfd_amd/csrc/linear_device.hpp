@@ -136,7 +136,7 @@ __device__ __forceinline__ void finish(const Linear& p, unsigned row, unsigned c
 // first, else they start 2 bytes in; the first word also holds the scale if at is 0.
 // (Loads that are not on 4 bytes take several times as long: 64 cycles each in the
 // few-row form.) The first word may begin 2 bytes before the block, the last
-// end 2 behind it; with `edge` (a matrix's first or last row) no byte
+// end 2 behind it; with `edge` (a matrix's first or last row, or rows that overlap) no byte
 // outside the block is read.
 template <int N>
 struct Q8Piece {
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
   WChunk wv[kIsQ8<W> || kDmaW ? 1 : kWItems];
   Q8Piece<16> qv[kIsQ8<W> ? kWItems : 1];
   uint32_t qd[kIsQ8<W> && !kScaled ? kWItems : 1];
-  const bool edge = col0 == 0 || col0 + COLS >= p.m;
+  const bool edge = col0 == 0 || col0 + COLS >= p.m || p.ldw < p.k;
   auto load = [&](unsigned k0) {
     if constexpr (!DMA) {
 #pragma unroll
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
       multiply(0);
     }
   };
-  if (kIsQ8<W> && (col0 == 0 || col0 + 16 >= p.m))
+  if (kIsQ8<W> && (col0 == 0 || col0 + 16 >= p.m || p.ldw < p.k))
     run(Const<1>{});
   else
     run(Const<0>{});
@@ -671,7 +671,7 @@ hipError_t launch_linear_form(const Linear& p, hipStream_t st) {
   constexpr unsigned kCus = 256;
   constexpr bool k32 = __is_same(T, float);
   auto count = [](unsigned n, unsigned by) { return (n + by - 1) / by; };
-  // n m <= 2^32: at most 2^24 + 2^21 workgroups of any form.
+  // n m <= 2^32: at most 2^22 workgroups of any form.
   auto few = [&](auto blocks) {
     constexpr int NB = decltype(blocks)::value;
     linear_few_kernel<T, W, GATED, NB><<<count(p.n, 16 * NB) * count(p.m, 16), 64 * kFewWaves, 0, st>>>(p);

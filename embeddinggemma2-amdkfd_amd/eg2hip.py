@@ -978,8 +978,8 @@ class ops:
         if key_rows == 1:
             k_row, v_row = kv_heads * d, kv_heads * d
         batch = q_offsets.numel() - 1
-        if batch < 0:
-            raise ValueError(f"{what}: no offsets")
+        if batch < 0 or sinks < 0 or longest < 0:
+            raise ValueError(f"{what}: no offsets, or sinks {sinks} or longest {longest} below 0")
         qo = cls._vector(q_offsets, what, "q_offsets", batch + 1, int32, device)
         ko = qo if k_offsets is q_offsets else cls._vector(k_offsets, what, "k_offsets", batch + 1, int32, device)
         kl = 0 if k_lengths is None else cls._vector(k_lengths, what, "k_lengths", batch, int32, device)

@@ -228,8 +228,11 @@ int eg2_hip_gemm_q8_geglu(const int8_t *xq, const float *xd, unsigned ldx, const
  * hipError_t code; hipErrorInvalidValue for a record that breaks a rule below,
  * with nothing launched. They allocate nothing, keep nothing from one call to
  * the next and can be captured into a HIP graph. Sums, softmax statistics and
- * norms are held in 32 bits; every result is rounded once to its type (the
- * softmax weights of 16-bit attention also, before they multiply the values).
+ * norms are held in 32 bits; every result is rounded once to its type. The
+ * softmax weights of 16-bit attention multiply the values as the sum of two of its
+ * type, or, in calls with many query rows, rounded to one. A sum of products must
+ * not pass fp32's range on its way; of Q8_0 weights and 16-bit activations the sum over a
+ * block's 32 values comes before the block's scale.
  * Strides count elements and are free for inputs (0 repeats a row); pointers lie on their
  * type's own alignment (Q8_0 blocks on 2 bytes). An output overlaps no input unless its
  * rule says so. */
@@ -284,7 +287,8 @@ int eg2_hip_linear_gated(const eg2_linear_gated_args *args, void *stream);
  * head stride + e. q_out and k_out may be q and k themselves with the same
  * strides. The weights ([d], fp32) may be NULL (1). A row whose position is not
  * in [0, table_rows) comes out as NaN. d: even, 2 to 512; rotary: even, at most d (0: no
- * rotation, table and pos may be NULL); rows: 1 to 2^24; at most 4096 heads in all. */
+ * rotation, table and pos may be NULL); rows: 1 to 2^24; at most 4096 heads, and 2^25
+ * rows times heads, in all. */
 typedef struct {
     void *q_out, *k_out;
     const void *q, *k;
@@ -313,13 +317,13 @@ int eg2_hip_heads_norm_rope(const eg2_heads_norm_rope_args *args, void *stream);
  * and v that may be touched. q, k, v and out are of `type`, F32, F16 or BF16;
  * d: a multiple of 8, 8 to 256; their pointers lie on 16 bytes and their strides are
  * multiples of 16 bytes. heads is a multiple of kv_heads, at most 4096. batch: 1 to 65535;
- * rows and key_rows: 1 to 2^31 - 1; rows heads at most 2^27, batch kv_heads 2^22. longest: the longest
+ * rows heads at most 2^27, key_rows 2^30, batch kv_heads 2^22. longest: the longest
  * sequence of keys (0: unknown), a hint: it chooses how the keys of few queries are
  * split over the GPU, which costs time or the order of sums, never a key. workspace: device memory of
  * at least eg2_hip_window_attention_workspace(args) bytes (which may be 0), 16-byte
  * aligned, used by this call until its kernels are done: two calls that may
  * run at the same time, and two captured graphs that may, have one each.
- * scale: finite. */
+ * scale: at most 2^127 in magnitude (0: equal weights). */
 typedef struct {
     void *out;
     const void *q, *k, *v;

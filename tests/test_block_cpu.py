@@ -117,7 +117,8 @@ def test_window_attention_refuses(eg2):
                    {"heads": 0}, {"kv_heads": 0}, {"heads": 5}, {"heads": 4098, "kv_heads": 2}, {"d": 0}, {"d": 60},
                    {"d": 264}, {"type": 8}, {"q": P + 8}, {"k": P + 4}, {"v": P + 2}, {"out": P + 8}, {"q_row": 260},
                    {"k_head": 68}, {"v_row": 132}, {"out_head": 4}, {"q_offsets": P + 2}, {"k_lengths": P + 1},
-                   {"scale": math.inf}, {"scale": math.nan}, {"q_row": 1 << 31}):
+                   {"scale": math.inf}, {"scale": math.nan}, {"scale": -3e38}, {"q_row": 1 << 31},
+                   {"key_rows": (1 << 30) + 1}, {"batch": 65535, "kv_heads": 65, "heads": 65}):
         assert entry(C.byref(attention_record(eg2, **change)), None) == INVALID, change
     assert entry(C.byref(attention_record(eg2, type=0, k_row=130)), None) == INVALID
     assert entry(None, None) == INVALID
@@ -168,6 +169,7 @@ def test_python_refuses(eg2):
         lambda: o.window_attention(f(4, 2, 8), f(4, 1, 8), f(5, 1, 8), i(2), i(2), f(4, 2, 8), 1.0),
         lambda: o.window_attention(f(4, 2, 8), f(4, 1, 8), f(4, 1, 8), i(2), i(3), f(4, 2, 8), 1.0),
         lambda: o.window_attention(f(4, 2, 8), f(4, 1, 8), f(4, 1, 8), f(2), i(2), f(4, 2, 8), 1.0),
+        lambda: o.window_attention(f(4, 2, 8), f(4, 1, 8), f(4, 1, 8), i(0), i(0), f(4, 2, 8), 1.0),
         lambda: o.window_attention(f(4, 2, 8), h(4, 1, 8), h(4, 1, 8), i(2), i(2), f(4, 2, 8), 1.0),
     ]
     for call in bad:
@@ -210,3 +212,26 @@ def test_reference_quantizer_and_products():
     y, off = R.linear(x, values, None, "gelu", None, torch.bfloat16)
     t = torch.nn.functional.gelu(torch.from_numpy(x @ values.T), approximate="tanh").numpy()
     assert np.abs(y - t).max() < 1e-12 and (off >= R.rounding(y, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("source", ["kernels_window.hip", "kernels_linear_f32.hip", "kernels_linear_bf16.hip"])
+def test_only_the_dma_uses_m0(tmp_path, source):
+    """The loads to LDS set M0 in inline asm and declare it clobbered: sound only while no
+    instruction of the compiler's reads it. Every mention of m0 in the compiled kernels is the asm's own write."""
+    import re
+    import shutil
+    import subprocess
+
+    hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+    if not shutil.which(hipcc):
+        pytest.skip("hipcc not available")
+    pkg = os.path.join(ROOT, "embeddinggemma2-amdkfd_amd")
+    out = tmp_path / "kernels.s"
+    subprocess.run([hipcc, "--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off",
+                    "-fhip-fp32-correctly-rounded-divide-sqrt", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                    "-mllvm", "-amdgpu-mfma-vgpr-form", "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(pkg, "csrc"),
+                    "--cuda-device-only", "-S", os.path.join(pkg, "csrc", source), "-o", str(out)],
+                   check=True, capture_output=True, timeout=600)
+    uses = [code for code in (line.split(";")[0] for line in out.read_text().splitlines()) if re.search(r"\bm0\b", code)]
+    other = [code for code in uses if not re.match(r"\s*s_mov_b32 m0, s\d+\s*$", code)]
+    assert uses and not other, other[:5]
