@@ -30,12 +30,16 @@ struct OtherThanQ8<T, Q8> {
   typedef T type;
 };
 
-// Loads at any alignment of the values (one instruction: global loads need none).
+// Loads and stores at any alignment of the values (one instruction: the global ones need none).
 template <class V>
 __device__ __forceinline__ V load_any(const void* p) {
   V v;
   __builtin_memcpy(&v, p, sizeof(V));
   return v;
+}
+template <class V>
+__device__ __forceinline__ void store_any(void* p, const V& v) {
+  __builtin_memcpy(p, &v, sizeof(V));
 }
 
 // The W values [k, k + kPer16<T>) of a row as they lie, zeros from `end` on, and as 16
@@ -53,7 +57,9 @@ struct Chunk {
       load(row, k);
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e) raw.v[e] = k + e < end ? row[min(k + e, end - 1)] : (W)0.0f;
+      for (int e = 0; e < N; ++e) raw.v[e] = row[min(k + e, end - 1)];  // all on their way at once
+#pragma unroll
+      for (int e = 0; e < N; ++e) raw.v[e] = k + e < end ? raw.v[e] : (W)0.0f;
     }
   }
   __device__ __forceinline__ uintx4 get() const {
@@ -88,32 +94,30 @@ __device__ __forceinline__ void finish(const Linear& p, unsigned row, unsigned c
   if (row >= p.n || col >= p.m) return;
   constexpr int N = COLS % kPer16<T> == 0 ? kPer16<T> : 4;  // values of a store
   static_assert(COLS % 4 == 0, "");
-  struct alignas(sizeof(T) * N) Some {
+  struct Some {
     T v[N];
   };
   T* y = static_cast<T*>(p.y) + row * p.ldy + col;
   const T* r = p.residual ? static_cast<const T*>(p.residual) + row * p.ldr + col : nullptr;
-  auto on = [](const void* q) { return reinterpret_cast<uintptr_t>(q) % sizeof(Some) == 0; };
-  const bool whole = col + COLS <= p.m && on(y) && on(r);
   float z[COLS];
 #pragma unroll
   for (int e = 0; e < COLS; ++e) {
     z[e] = activate<ACT>(a[e] + a_bias.v[e]);
     if constexpr (GATED) z[e] = z[e] * (b[e] + b_bias.v[e]);
   }
-  if (whole) {
+  if (col + COLS <= p.m) {
 #pragma unroll
     for (int c = 0; c < COLS; c += N) {
       if constexpr (!GATED)
         if (r) {
-          const Some s = *reinterpret_cast<const Some*>(r + c);
+          const Some s = load_any<Some>(r + c);
 #pragma unroll
           for (int e = 0; e < N; ++e) z[c + e] = z[c + e] + to_float(s.v[e]);
         }
       Some out;
 #pragma unroll
       for (int e = 0; e < N; ++e) out.v[e] = (T)z[c + e];
-      *reinterpret_cast<Some*>(y + c) = out;
+      store_any(y + c, out);
     }
   } else {
     if constexpr (!GATED)
@@ -352,27 +356,44 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
       }
       return;
     }
-    auto piece = [&](const unsigned char* base, uint32_t off, unsigned chunk, uint32_t to, unsigned char* place) {
-      if (k0 + N * chunk + N <= p.k)
-        dma16(base + k0 * sizeof(T), off, to);
-      else {
-        Chunk<T, T> c;
-        c.load(reinterpret_cast<const T*>(base + off - 16 * chunk), k0 + N * chunk, p.k);
-        *reinterpret_cast<uintx4*>(place + 16 * lane) = c.get();
-      }
+    // Chunk c of a row as far as it lies before k: straight to LDS if it does as a whole.
+    auto whole = [&](unsigned chunk) { return k0 + N * chunk + N <= p.k; };
+    auto part = [&](const unsigned char* base, uint32_t off, unsigned chunk) {
+      Chunk<T, T> c;
+      c.load(reinterpret_cast<const T*>(base + off - 16 * chunk), k0 + N * chunk, p.k);
+      return c;
     };
+    const unsigned xchunk = (lane & 7) ^ (lane >> 3);
+    auto wchunk = [&](int i) { return (lane & 7) ^ weight_key<JBG>(8 * (kWDma * wave + i) + (lane >> 3)); };
+    auto wfrom = [&](int i) { return wbase[GATED && 8 * (kWDma * wave + i) >= COLS]; };
+    Chunk<T, T> xs[DMA ? kXDma : 1], ws[kDmaW ? kWDma : 1];
     if constexpr (DMA) {
 #pragma unroll
-      for (int i = 0; i < kXDma; ++i)
-        piece(xbase, xoff[i], (lane & 7) ^ (lane >> 3), to_x + 1024 * i, lds.x[buf] + 1024 * (kXDma * wave + i));
+      for (int i = 0; i < kXDma; ++i) {
+        if (whole(xchunk))
+          dma16(xbase + k0 * sizeof(T), xoff[i], to_x + 1024 * i);
+        else
+          xs[i] = part(xbase, xoff[i], xchunk);
+      }
     }
     if constexpr (kDmaW) {
 #pragma unroll
       for (int i = 0; i < kWDma; ++i) {
-        const int at = kWDma * wave + i;
-        piece(wbase[GATED && 8 * at >= COLS], woff[i], (lane & 7) ^ weight_key<JBG>(8 * at + (lane >> 3)), to_w + 1024 * i,
-              lds.w[buf] + 1024 * at);
+        if (whole(wchunk(i)))
+          dma16(wfrom(i) + k0 * sizeof(T), woff[i], to_w + 1024 * i);
+        else
+          ws[i] = part(wfrom(i), woff[i], wchunk(i));
       }
+    }
+    if constexpr (DMA) {
+#pragma unroll
+      for (int i = 0; i < kXDma; ++i)
+        if (!whole(xchunk)) *reinterpret_cast<uintx4*>(lds.x[buf] + 1024 * (kXDma * wave + i) + 16 * lane) = xs[i].get();
+    }
+    if constexpr (kDmaW) {
+#pragma unroll
+      for (int i = 0; i < kWDma; ++i)
+        if (!whole(wchunk(i))) *reinterpret_cast<uintx4*>(lds.w[buf] + 1024 * (kWDma * wave + i) + 16 * lane) = ws[i].get();
     }
   };
 
