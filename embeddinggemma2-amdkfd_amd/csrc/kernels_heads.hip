@@ -141,7 +141,8 @@ hipError_t launch_heads_norm_rope(const eg2_heads_norm_rope_args& a, hipStream_t
                       on16(a.q_weight, 0, 0) && on16(a.k_weight, 0, 0) && on16(a.table, 0, 0);
     if (!wide) return go<T, 1, 64, 4, 1>(a, st);
     const unsigned chunks = a.d / 2 / V;  // of each half, at most 64
-    // Four heads to a group where that leaves a wave for every SIMD.
+    // Four heads to a group where that leaves a wave for every SIMD: 8192 rows of 16 + 4 x 128 bf16 20 us, 4.3 TB/s
+    // (one head: 55 us); with fewer rows one (2011 of 3 + 1 x 256 fp32: 5.3 us).
     auto by = [&](auto lanes) {
       constexpr int L = decltype(lanes)::value;
       const uint64_t heads = (uint64_t)a.rows * (a.q_heads + a.k_heads);

@@ -21,6 +21,13 @@
 // (weights up to 2^8 lose nothing in any type), which spares most of the
 // rescaling of the sums.
 //
+// Bound: causal 8192 bf16 of 16 + 4 x 128 takes 238 us, 865 TFLOP/s; a wave's
+// products, its softmax and its LDS reads each take about a third of that, and two waves a
+// SIMD hide them behind each other in part (the matrix units work 42 % of the cycles). One token over caches:
+// the keys' and values' bytes (24 caches of 6000 x 4 x 128 bf16 with a window of 2048: 21.3 us and 3.9
+// of the join, 4.0 TB/s; 48 of 8192 x 8 x 128: 304 us, 5.3 TB/s). Short texts: the
+// chain of a tile's keys and the launch (16 texts of 128 bf16, 3 + 1 x 256: 11.4 us).
+//
 // A key that a row does not see has weight 0, but 0 times an infinite or NaN
 // value is NaN: where some row of the wave does not see a tile's keys, the values
 // are looked at first, and a tile with such a value goes key by key (add_by_key).
@@ -619,13 +626,21 @@ Plan plan(const Args& a) {
     const uint64_t window = (uint64_t)a.left + a.sinks + (a.right >= 0 ? (uint64_t)a.right + 1 : longest);
     span = window < span ? window : span;
   }
+  // The more rows a tile has, the less often keys are read; but the GPU needs a workgroup for most of
+  // its CUs. us by tiles of 128, 64, 32 and 16 rows: bf16 8 x 1024 of 3 + 1 x 256, window 512: 42, 56, 67, -;
+  // 4 x 1024 40, 31, 46, 72; 1 x 2048 -, 28.5, 24.9, 49; 16 x 128 -, 15.8, 13.4, 20.7; causal 3 x 1024 of 16 + 4 x 128
+  // 45, 50, 75, -; 1 x 1024 33, 22, 27, 42; 1 x 2048 57, 44, 73, -; fp32 4 x 1024 -, 101, 126, 191; 1 x 2048 -, 100, 65, 127.
   if (pairs > kFewRows * busy) {
     const bool uneven = a.right >= 0 && span > longest / 2;  // causal: the first rows have few keys, the last all
     if (a.type != EG2_TYPE_F32 && groups(128) >= (uneven ? 320 : 144)) return Plan{128, 1};
     if (groups(64) >= 144) return Plan{64, 1};
     if (groups(32) >= 144) return Plan{32, 1};
   }
-  // One round of workgroups: two to a CU where a row of keys takes 128 bytes, one beyond.
+  // The keys split over one round of workgroups: two to a CU where a row of keys takes 128 bytes, one
+  // beyond (24 caches at 192 workgroups 28 us, at 480 39). Each at least 64 keys (1 x 8192 x 256: 13.8 us; 256 keys 17, 512 23),
+  // and none below 512, where the join costs more (300 keys: split 8.8 us, whole 7.3; 1000: 10.8, 14.9). Tiles
+  // of 32 and 64 rows are not split: their sums make the join too long (300 rows over 3000: 34 us, whole
+  // 36; 500 over 1000: 32, 20).
   const uint64_t row = (a.d <= 64 ? 64u : a.d <= 128 ? 128u : 256u) * (a.type == EG2_TYPE_F32 ? 4u : 2u);
   uint64_t splits = (row <= 128 ? 2 * kCus : kCus) / groups(kFewRows);
   if (splits > span / 64) splits = span / 64;

@@ -172,12 +172,20 @@ struct Q8Piece {
 // ------------------------------------------------------------------ tiles
 //
 // BM rows of x times BN rows of the weights (of a gated pair BN / 2 of each
-// matrix) per workgroup of WM x WN waves, each 16 x 16 blocks over its
-// part, or of WK times as many, each share over every WK-th slice of k, added at the end. Slices of 128 bytes of every row go through NBUF LDS buffers, all but one
-// on their way while one is multiplied. The 16-byte chunks of a row are
-// swizzled so that the 16 rows of a fragment read lie on distinct banks. Rows on
-// 4 bytes go straight to LDS (DMA), others and what has to be decoded through
-// registers.
+// matrix) per workgroup of WM x WN waves, each 16 x 16 blocks over its part, or
+// of WK times as many, each share over every WK-th slice of k, added at the
+// end. Slices of 128 bytes of every row go through NBUF LDS buffers, all but one
+// on their way while one is multiplied. The 16-byte chunks of a row are swizzled
+// so that no read waits for LDS's banks (counted: 0 conflicts). Rows on 4 bytes go
+// straight to LDS (DMA), others and what has to be decoded through registers.
+//
+// Bound: large products by the matrix units. 4096 x 2048 x 8192 bf16 with bias
+// and GELU takes 127 us, 1080 TFLOP/s, of which 54 % of the cycles the matrix units work
+// (a product of 8192^3 by the installed library, no epilogue: 1244 TFLOP/s; its own
+// of this size, no epilogue: 103 us). Products that leave most CUs one or two tiles, by how fast a
+// CU takes slices from L2 (22 to 26 bytes a cycle): 2048 x 768 x 1152 gated bf16 14 us.
+// Deeper buffers (3, 4 slices of 128 or 256 rows) and tiles of 128 x 192 where those
+// would save a round of workgroups measured within 3 % of these.
 constexpr int kRowBytes = 128, kChunks = kRowBytes / 16;
 
 // A wave's block j of JBG, lane i: which of its 16 JBG weight rows it feeds, so
@@ -504,6 +512,11 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 // matrix) per workgroup of eight waves, which take every eighth step of k
 // and add their sums through LDS: the weights come straight from memory in
 // the order of the operand, and every workgroup's chain is an eighth of k.
+//
+// Bound: the weights' bytes once there are some (1 x 4096 x 8192 bf16: 14.2 us, 4.7
+// TB/s; 4 x 2048 x 8192 gated Q8_0: 15 us, 2.4 TB/s, where unpacking the blocks counts as well:
+// 40 VALU instructions a step), below that the launch and one chain of loads (1 x 768 x 768:
+// 3.7 us).
 constexpr int kFewWaves = 8;
 
 template <class T, class W, bool EDGE>
@@ -698,12 +711,19 @@ hipError_t launch_linear_form(const Linear& p, hipStream_t st) {
     linear_few_kernel<T, W, GATED, NB><<<count(p.n, 16 * NB) * count(p.m, 16), 64 * kFewWaves, 0, st>>>(p);
     return hipGetLastError();
   };
+  // Few rows, or so few blocks of 16 x 16 that they are one round of the GPU's
+  // workgroups (two to a CU). Then more row blocks to a workgroup instead of more
+  // rounds; fp32 goes on so where 16-bit types are better off with tiles. us by 1, 2 and 4 blocks and by
+  // tiles: 45 x 768 x 1280 fp32 Q8_0 6.6, 8.4, 10.6, 20; 64 x 768 x 768 fp32 5.9, 7.6, 10.9, 17;
+  // 300 x 768 x 768 fp32 15.8, 13.4, 12.1, 20.6; 32 x 2048 x 2048 bf16 6.8, 8.6, 9.6, 9.3;
+  // 100 x 768 x 768 bf16 5.6, 5.2, 6.6, 6.6; 256 x 768 x 2304 bf16 16, 13.9, 14.1, 6.8.
   const uint64_t down16 = count(p.n, 16), across16 = count(p.m, 16);
   if (p.n <= 16 || down16 * across16 <= 2 * kCus) return few(Const<1>{});
   if (p.n <= 32 || (k32 && (down16 + 1) / 2 * across16 <= 2 * kCus)) return few(Const<2>{});
   if (k32 && (down16 + 3) / 4 * across16 <= 2 * kCus) return few(Const<4>{});
   constexpr unsigned kSmallCols = GATED ? 32 : 64, kLargeCols = GATED ? 64 : 128;
-  // Straight to LDS where rows lie on 4 bytes, and a tile's within 2^31.
+  // Straight to LDS where rows lie on 4 bytes (333 x 1152 x 768 f16: 7.5 us; 1151, whose rows do
+  // not: 12.7), and a tile's within 2^31 bytes of each other.
   bool dma = on4(p.x, p.ldx, sizeof(T));
   if constexpr (__is_same(T, W))
     for (int z = 0; z < (GATED ? 2 : 1); ++z) dma = dma && on4(p.w[z], p.ldw, sizeof(T));
@@ -718,12 +738,20 @@ hipError_t launch_linear_form(const Linear& p, hipStream_t st) {
       linear_tile_kernel<T, W, GATED, false, B, B, WM, WN, WK, 2><<<groups, 64 * WM * WN * WK, 0, st>>>(p);
     return hipGetLastError();
   };
+  // The largest tile of which there is one for every CU: it reads its operands least often. us by
+  // tiles of 64, 128 and 256: 4096 x 2048 x 8192 bf16 250, 151, 128; 4096^3 223, 136, 120; gated 4096 x 2048 x 4096
+  // 213, 137, 118; 2048 x 768 x 2304 f16 22, 18, 28; 1000 x 1150 x 2001 20, 30, 55; fp32 4096 x 2048 x 2048
+  // 289, 252 (2048 x 768 x 1152, too few: 49, 58). 16-bit activations on Q8_0 stay with 64, whose scales
+  // leave it registers (2048 x 768 x 2304 32, 50; 4096 x 2048 x 4096 169, 229).
   if constexpr (kSame && !k32)
     if (count(p.n, 256) * count(p.m, 2 * kLargeCols) >= kCus)
       return tiles(Const<256>{}, Const<2>{}, Const<4>{}, Const<1>{}, Const<2>{});
   if constexpr (!kIsQ8<W> || k32)
     if (count(p.n, 128) * count(p.m, kLargeCols) >= kCus)
       return tiles(Const<128>{}, Const<2>{}, Const<2>{}, Const<1>{}, Const<2>{});
+  // Fewer tiles than CUs: four shares of k to a workgroup. us of 1, 2 and 4 shares: 512 x 768 x 768 bf16 7.3, 6.7, 6.9;
+  // 128 x 2048 x 2048 12.9, 13.8, 11.9; 64 x 4096 x 4096 22, 24, 20; 300 x 768 x 1152 f16 Q8_0 13.6, 10.4, 9.1; with more
+  // tiles one (1000 x 1150 x 2001 20.2, 19.6, 24.5), or two of fp32 (2048 x 768 x 1152 50, 47, 51).
   if (count(p.n, 64) * count(p.m, kSmallCols) < kCus)
     return tiles(Const<64>{}, Const<2>{}, Const<2>{}, Const<4>{}, Const<2>{});
   return tiles(Const<64>{}, Const<2>{}, Const<2>{}, Const<k32 ? 2 : 1>{}, Const<k32 ? 2 : 4>{});
