@@ -509,11 +509,11 @@ __global__ void __launch_bounds__(64 * WM * WN * WK) linear_tile_kernel(Linear p
 // ------------------------------------------------------------------ few rows
 //
 // 16 NB rows of x times 16 rows of the weights (of a gated pair of each
-// matrix) per workgroup of eight waves, which take every eighth step of k
+// matrix) per workgroup of eight waves, which take an eighth of k's steps each
 // and add their sums through LDS: the weights come straight from memory in
 // the order of the operand, and every workgroup's chain is an eighth of k.
 //
-// Bound: the weights' bytes once there are some (1 x 4096 x 8192 bf16: 14.2 us, 4.7
+// Bound: the weights' bytes once there are some (1 x 4096 x 8192 bf16: 13.5 us, 5.0
 // TB/s; 4 x 2048 x 8192 gated Q8_0: 15 us, 2.4 TB/s, where unpacking the blocks counts as well:
 // 40 VALU instructions a step), below that the launch and one chain of loads (1 x 768 x 768:
 // 3.7 us).
@@ -566,6 +566,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
   // Steps on their way: of a pair two, so that its registers leave room for as many
   // waves as one matrix has with four (4 x 2048 x 8192 Q8_0: 16.7 us, 18.9 with four).
   constexpr int kDepth = NB * G >= 4 || GATED ? 2 : 4;
+  constexpr int kSlots = GATED && NB == 1 ? 3 : kDepth;  // all the steps of a wave that has no more, at once (1 x 768 x 1152 pairs 8 % less)
+  // A wave takes a run of steps, or every eighth: runs keep a row's memory together (1 x 4096 x 4096 fp32
+  // 13.9 us, 16.2 by eighths; 1 x 4096 x 8192 bf16 13.5, 14.2), while Q8_0 blocks share their cache lines with the
+  // next steps, which eighths fetch at the same time (4 x 2048 x 8192 gated 16.9, 17.1 by runs; 1 x 4096 x 4096 12.1, 12.2).
+  constexpr bool kRuns = !kIsQ8<W> && !GATED;
   __shared__ floatx4 part[kFewWaves][G][NB][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, r = lane & 15;
@@ -592,8 +597,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
     for (int i = 0; i < NB; ++i) acc[z][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
   auto run = [&](auto edge) {
     constexpr bool EDGE = decltype(edge)::value != 0;
-    FewWeights<T, W, EDGE> w[kDepth][G];
-    Chunk<T, T> x[kDepth][NB][kChunk];
+    FewWeights<T, W, EDGE> w[kSlots][G];
+    Chunk<T, T> x[kSlots][NB][kChunk];
     auto multiply = [&](int slot) {
 #pragma unroll
       for (int z = 0; z < G; ++z) {
@@ -614,11 +619,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
         }
       }
     };
-    // The wave's whole steps: wave, wave + 8, .. The loop's loads stand in no
-    // branch (past the last step it is loaded again), so that a step waits for its own alone.
-    const unsigned steps = p.k / 32, mine = steps > (unsigned)wave ? (steps - wave + kFewWaves - 1) / kFewWaves : 0;
+    // The wave's whole steps. The loop's loads stand in no branch (past the last
+    // step it is loaded again), so that a step waits for its own alone.
+    const unsigned steps = p.k / 32, begin = kRuns ? steps * wave / kFewWaves : wave;
+    const unsigned mine = kRuns ? steps * (wave + 1) / kFewWaves - begin : steps > begin ? (steps - begin + kFewWaves - 1) / kFewWaves : 0;
     auto load = [&](int slot, unsigned n) {
-      const unsigned k = 32 * (wave + kFewWaves * min(n, mine - 1));
+      const unsigned k = 32 * (begin + (kRuns ? 1 : kFewWaves) * min(n, mine - 1));
 #pragma unroll
       for (int z = 0; z < G; ++z) w[slot][z].load(wrow[z], k, g);
 #pragma unroll
@@ -626,7 +632,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
 #pragma unroll
         for (int c = 0; c < kChunk; ++c) x[slot][i][c].load(xrow[i], k + kPer16<T> * (4 * c + g));
     };
-    if (mine > kDepth) {
+    if (mine > kSlots) {
 #pragma unroll
       for (int s = 0; s < kDepth; ++s) load(s, s);
       unsigned n = 0;
@@ -642,14 +648,14 @@ __global__ void __launch_bounds__(64 * kFewWaves) linear_few_kernel(Linear p) {
         if (n + s < mine) multiply(s);
     } else {
 #pragma unroll
-      for (int s = 0; s < kDepth; ++s)
+      for (int s = 0; s < kSlots; ++s)
         if (s < (int)mine) load(s, s);
 #pragma unroll
-      for (int s = 0; s < kDepth; ++s)
+      for (int s = 0; s < kSlots; ++s)
         if (s < (int)mine) multiply(s);
     }
     // The values past the last whole step.
-    if (p.k % 32 != 0 && steps % kFewWaves == (unsigned)wave) {
+    if (p.k % 32 != 0 && wave == (int)(kRuns ? 0 : steps % kFewWaves)) {
 #pragma unroll
       for (int z = 0; z < G; ++z) w[0][z].load(wrow[z], 32 * steps, g, p.k);
 #pragma unroll
