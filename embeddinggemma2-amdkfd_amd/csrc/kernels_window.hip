@@ -235,8 +235,8 @@ window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out
 
   auto compute = [&](const unsigned char* ks, int from, int end) {
     const unsigned char* vs = ks + kTile;
-    // Sixteen keys from `key0` on, their weights in lds_w, their values at `rows`: each where it is seen alone.
-    auto add_by_key = [&](const unsigned char* rows, int key0) {
+    // Adds sixteen keys from `key0` on, their weights in lds_w, their values at `rows`: each where it is seen alone.
+    auto add_by_key = [&](floatx4 (&sum)[QB][OB], const unsigned char* rows, int key0) {
 #pragma unroll 1
       for (int j = 0; j < 16; ++j)
 #pragma unroll
@@ -252,7 +252,7 @@ window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out
               const int dim = k32 ? 64 * (o / 4) + 16 * g + 4 * e + o % 4 : 16 * o + 4 * g + e;
               // the tile's rows go by sixteen, so row j has value_swizzle(j)
               const T f = *reinterpret_cast<const T*>(rows + j * RB + 16 * ((dim / N) ^ value_swizzle(j)) + dim % N * sizeof(T));
-              acc[i][o][e] = __builtin_fmaf(w, to_float(f), acc[i][o][e]);
+              sum[i][o][e] = __builtin_fmaf(w, to_float(f), sum[i][o][e]);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
@@ -360,15 +360,24 @@ window_attention_kernel(Args p, unsigned slots, unsigned splits, float* part_out
           for (int o = 0; o < OB; ++o) odd |= non_finite_bits<T>(value16(kp, o, mine_r));
       }
       asm volatile("" ::: "memory");  // read again below, not kept in registers
-      if (__any(odd != 0)) {  // key by key
+      if (__any(odd != 0)) {  // key by key, to sums of their own: acc is moved to no other registers behind the products
+        floatx4 sum[QB][OB];
+#pragma unroll
+        for (int i = 0; i < QB; ++i)
+#pragma unroll
+          for (int o = 0; o < OB; ++o) sum[i][o] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
           for (int i = 0; i < QB; ++i) *reinterpret_cast<floatx4*>(&lds_w[wave][16 * i + r][4 * g]) = sc[i][kb];
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          add_by_key(vs + 16 * kb * RB, from + 16 * kb);
+          add_by_key(sum, vs + 16 * kb * RB, from + 16 * kb);
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
+#pragma unroll
+        for (int i = 0; i < QB; ++i)
+#pragma unroll
+          for (int o = 0; o < OB; ++o) acc[i][o] = acc[i][o] + sum[i][o];
         return;
       }
     }
