@@ -21,12 +21,12 @@
 // (weights up to 2^8 lose nothing in any type), which spares most of the
 // rescaling of the sums.
 //
-// Bound: causal 8192 bf16 of 16 + 4 x 128 takes 238 us, 865 TFLOP/s; a wave's
+// Bound: causal 8192 bf16 of 16 + 4 x 128 takes 230 to 240 us, 860 to 900 TFLOP/s; a wave's
 // products, its softmax and its LDS reads each take about a third of that, and two waves a
 // SIMD hide them behind each other in part (the matrix units work 42 % of the cycles). One token over caches:
-// the keys' and values' bytes (24 caches of 6000 x 4 x 128 bf16 with a window of 2048: 21.3 us and 3.9
-// of the join, 4.0 TB/s; 48 of 8192 x 8 x 128: 304 us, 5.3 TB/s). Short texts: the
-// chain of a tile's keys and the launch (16 texts of 128 bf16, 3 + 1 x 256: 11.4 us).
+// the keys' and values' bytes (24 caches of 6000 x 4 x 128 bf16 with a window of 2048: 20.8 us and 3.6
+// of the join, 4.1 TB/s; 48 of 8192 x 8 x 128: 304 us, 5.3 TB/s). Short texts: the
+// chain of a tile's keys and the launch (16 texts of 128 bf16, 3 + 1 x 256: 11 us).
 //
 // A key that a row does not see has weight 0, but 0 times an infinite or NaN
 // value is NaN: where some row of the wave does not see a tile's keys, the values

@@ -180,7 +180,7 @@ struct Q8Piece {
 // straight to LDS (DMA), others and what has to be decoded through registers.
 //
 // Bound: large products by the matrix units. 4096 x 2048 x 8192 bf16 with bias
-// and GELU takes 127 us, 1080 TFLOP/s, of which 54 % of the cycles the matrix units work
+// and GELU takes 123 to 127 us, 1080 to 1120 TFLOP/s, of which 55 % of the cycles the matrix units work
 // (a product of 8192^3 by the installed library, no epilogue: 1244 TFLOP/s; its own
 // of this size, no epilogue: 103 us). Products that leave most CUs one or two tiles, by how fast a
 // CU takes slices from L2 (22 to 26 bytes a cycle): 2048 x 768 x 1152 gated bf16 14 us.
